@@ -926,6 +926,14 @@ fa_status check_row_view(const char *name, const void *p, int64_t ld, int32_t co
                     (long long)ld, cols);
     return FA_OK;
 }
+// A row view that needs its element's alignment only; NULL is fine for no rows.
+fa_status check_any_view(const char *name, const void *p, int64_t ld, int64_t rows, int64_t cols, int32_t dtype) {
+    if (!p && rows > 0) return fail(FA_ERR_INVALID_ARG, "%s is NULL", name);
+    if (!aligned(p, dtype_bytes(dtype))) return fail(FA_ERR_INVALID_ARG, "%s is misaligned", name);
+    if (rows > 1 && ld < cols)
+        return fail(FA_ERR_INVALID_ARG, "%s: ld %lld must be >= cols %lld", name, (long long)ld, (long long)cols);
+    return FA_OK;
+}
 fa_status check_vec(const char *name, const void *p) {
     if (!p || !aligned(p, 16)) return fail(FA_ERR_INVALID_ARG, "%s is NULL or not 16-byte aligned", name);
     return FA_OK;
@@ -1076,6 +1084,89 @@ fa_status fa_ln_mod_bwd_gate(const fa_ln_mod_bwd_gate_args *a, void *stream) {
     p.ldgdx = a->ldgdx;
     const hipError_t e = fa::launch_ln_mod_bwd(p, w->fwd.dtype, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "layer-norm-mod backward launch");
+    return ok();
+}
+
+static fa_status check_layer_norm(const fa_layer_norm_args *a) {
+    if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F32) return fail(FA_ERR_INVALID_ARG, "unknown dtype %d", a->dtype);
+    if (a->param_dtype != FA_DTYPE_BF16 && a->param_dtype != FA_DTYPE_F32)
+        return fail(FA_ERR_INVALID_ARG, "unknown param_dtype %d", a->param_dtype);
+    if (a->rows < 0 || a->cols < 1) return fail(FA_ERR_INVALID_ARG, "rows %d / cols %d: need rows >= 0, cols >= 1", a->rows, a->cols);
+    if (a->cols > FA_LAYER_NORM_MAX_COLS)
+        return fail(FA_ERR_UNSUPPORTED, "cols %d: this build implements up to %d", a->cols, FA_LAYER_NORM_MAX_COLS);
+    FA_TRY(check_any_view("x", a->x, a->ldx, a->rows, a->cols, a->dtype));
+    if (!a->weight || !aligned(a->weight, dtype_bytes(a->param_dtype)))
+        return fail(FA_ERR_INVALID_ARG, "weight is NULL or misaligned");
+    return FA_OK;
+}
+
+static fa::LayerNormParams layer_norm_params(const fa_layer_norm_args *a) {
+    fa::LayerNormParams p{};
+    p.x = a->x;
+    p.ldx = a->ldx;
+    p.w = a->weight;
+    p.b = a->bias;
+    p.y = a->y;
+    p.ldy = a->ldy;
+    p.mean = a->mean;
+    p.rstd = a->rstd;
+    p.N = a->rows;
+    p.C = a->cols;
+    p.eps = a->eps;
+    return p;
+}
+
+fa_status fa_layer_norm_fwd(const fa_layer_norm_args *a, void *stream) {
+    if (!a) return fail(FA_ERR_INVALID_ARG, "args is NULL");
+    FA_TRY(check_layer_norm(a));
+    if (!(a->eps > 0.f) || !isfinite(a->eps)) return fail(FA_ERR_INVALID_ARG, "eps must be finite and > 0");
+    if (a->bias && !aligned(a->bias, dtype_bytes(a->param_dtype))) return fail(FA_ERR_INVALID_ARG, "bias is misaligned");
+    FA_TRY(check_any_view("y", a->y, a->ldy, a->rows, a->cols, a->dtype));
+    if ((a->mean == nullptr) != (a->rstd == nullptr) && a->rows > 0)
+        return fail(FA_ERR_INVALID_ARG, "mean and rstd must both be given or both NULL");
+    if (!aligned(a->mean, 4) || !aligned(a->rstd, 4)) return fail(FA_ERR_INVALID_ARG, "mean/rstd misaligned");
+    FA_TRY(init_current());
+    const hipError_t e = fa::launch_layer_norm_fwd(layer_norm_params(a), a->dtype, a->param_dtype,
+                                                   static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "layer-norm launch");
+    return ok();
+}
+
+size_t fa_layer_norm_bwd_workspace_size(const fa_layer_norm_bwd_args *a) {
+    if (!a || a->fwd.rows < 0 || a->fwd.cols < 1 || a->fwd.cols > FA_LAYER_NORM_MAX_COLS) return 0;
+    return fa::layer_norm_bwd_workspace_bytes(a->fwd.rows, a->fwd.cols);
+}
+
+fa_status fa_layer_norm_bwd(const fa_layer_norm_bwd_args *a, void *stream) {
+    if (!a) return fail(FA_ERR_INVALID_ARG, "args is NULL");
+    const fa_layer_norm_args *f = &a->fwd;
+    FA_TRY(check_layer_norm(f));
+    if (f->rows > 0 && (!f->mean || !f->rstd))
+        return fail(FA_ERR_INVALID_ARG, "mean and rstd (from the forward) are required");
+    if (!aligned(f->mean, 4) || !aligned(f->rstd, 4)) return fail(FA_ERR_INVALID_ARG, "mean/rstd misaligned");
+    FA_TRY(check_any_view("dy", a->dy, a->lddy, f->rows, f->cols, f->dtype));
+    FA_TRY(check_any_view("dx", a->dx, a->lddx, f->rows, f->cols, f->dtype));
+    if (a->dres) FA_TRY(check_any_view("dres", a->dres, a->ldres, f->rows, f->cols, f->dtype));
+    if (!aligned(a->dweight, 4) || !aligned(a->dbias, 4)) return fail(FA_ERR_INVALID_ARG, "dweight/dbias misaligned");
+    const bool grads = a->dweight || a->dbias;
+    if (grads) {
+        const size_t need = fa::layer_norm_bwd_workspace_bytes(f->rows, f->cols);
+        if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need)
+            return fail(FA_ERR_INVALID_ARG, "workspace is NULL, not 256-byte aligned, or smaller than %zu bytes", need);
+    }
+    FA_TRY(init_current());
+    fa::LayerNormParams p = layer_norm_params(f);
+    p.dy = a->dy;
+    p.lddy = a->lddy;
+    p.dres = a->dres;
+    p.ldres = a->ldres;
+    p.dx = a->dx;
+    p.lddx = a->lddx;
+    p.dw = a->dweight;
+    p.db = a->dbias;
+    p.part = grads ? static_cast<float *>(a->workspace) : nullptr;
+    const hipError_t e = fa::launch_layer_norm_bwd(p, f->dtype, f->param_dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "layer-norm backward launch");
     return ok();
 }
 

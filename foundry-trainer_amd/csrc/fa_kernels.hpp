@@ -178,6 +178,30 @@ struct LnModParams {
 hipError_t launch_ln_mod_fwd(const LnModParams &p, int dtype, hipStream_t s);
 hipError_t launch_ln_mod_bwd(const LnModParams &p, int dtype, hipStream_t s);
 
+// Layer norm with weight and bias over [N, C] rows (C <= 32768, any strides).
+struct LayerNormParams {
+    const void *x;
+    int64_t ldx;
+    const void *w, *b;   // [C] of the parameters' dtype; b may be null
+    void *y;
+    int64_t ldy;
+    float *mean, *rstd;  // [N]: written by fwd (optional), read by bwd
+    const void *dy;      // bwd
+    int64_t lddy;
+    const void *dres;    // bwd: added to dx (optional)
+    int64_t ldres;
+    void *dx;
+    int64_t lddx;
+    float *dw, *db;      // bwd: [C], either may be null
+    float *part;         // bwd: partial rows of dw and db; null: neither is wanted
+    int N, C;
+    float eps;
+    int G;  // waves per row, set by the launcher
+};
+size_t layer_norm_bwd_workspace_bytes(int N, int C);
+hipError_t launch_layer_norm_fwd(const LayerNormParams &p, int dtype, int wdtype, hipStream_t s);
+hipError_t launch_layer_norm_bwd(const LayerNormParams &p, int dtype, int wdtype, hipStream_t s);
+
 // Elementwise ops over an [N, C] view (C % 8 == 0): 0 gated residual
 // y = x + g*b, 1 y = gelu(b), 2 y = x * gelu'(b), 3 y = silu(b).
 struct EltParams {

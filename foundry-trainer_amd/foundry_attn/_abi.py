@@ -35,6 +35,7 @@ EXPORTED = [
     "fa_lora_down", "fa_lora_up", "fa_lora_grad", "fa_lora_grad_workspace_size",
     "fa_lora_grad_many", "fa_lora_grad_many_workspace_size",
     "fa_gated_ln_mod_fwd", "fa_ln_mod_bwd_gate", "fa_gemm_bf16",
+    "fa_layer_norm_fwd", "fa_layer_norm_bwd", "fa_layer_norm_bwd_workspace_size",
 ]
 
 
@@ -134,6 +135,22 @@ class GatedLnModArgs(ctypes.Structure):
 
 class LnModBwdGateArgs(ctypes.Structure):
     _fields_ = [("bwd", LnModBwdArgs), ("g", ctypes.c_void_p), ("gdx", ctypes.c_void_p), ("ldgdx", ctypes.c_int64)]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("rows", ctypes.c_int32),
+        ("cols", ctypes.c_int32), ("eps", ctypes.c_float), ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+        ("mean", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+    ]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", LayerNormArgs), ("dy", ctypes.c_void_p), ("lddy", ctypes.c_int64),
+                ("dres", ctypes.c_void_p), ("ldres", ctypes.c_int64), ("dx", ctypes.c_void_p),
+                ("lddx", ctypes.c_int64), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class RowsArgs(ctypes.Structure):
@@ -264,10 +281,13 @@ def lib() -> ctypes.CDLL:
                      ("fa_gelu_bwd", RowsArgs), ("fa_silu", RowsArgs), ("fa_adamw_step", AdamwArgs),
                      ("fa_swiglu_fwd", SwigluArgs), ("fa_swiglu_bwd", SwigluBwdArgs),
                      ("fa_lora_down", LoraDownArgs), ("fa_lora_up", LoraUpArgs), ("fa_lora_grad", LoraGradArgs),
-                     ("fa_gemm_bf16", GemmArgs)):
+                     ("fa_gemm_bf16", GemmArgs), ("fa_layer_norm_fwd", LayerNormArgs),
+                     ("fa_layer_norm_bwd", LayerNormBwdArgs)):
         fn = getattr(L, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
+    L.fa_layer_norm_bwd_workspace_size.restype = ctypes.c_size_t
+    L.fa_layer_norm_bwd_workspace_size.argtypes = [ctypes.POINTER(LayerNormBwdArgs)]
     L.fa_lora_grad_workspace_size.restype = ctypes.c_size_t
     L.fa_lora_grad_workspace_size.argtypes = [ctypes.POINTER(LoraGradArgs)]
     L.fa_lora_grad_many.restype = ctypes.c_int

@@ -61,6 +61,8 @@ _pack_ln_bwd_gate = _abi.packer(_abi.LnModBwdGateArgs)
 _pack_rows = _abi.packer(_abi.RowsArgs)
 _pack_swiglu = _abi.packer(_abi.SwigluArgs)
 _pack_swiglu_bwd = _abi.packer(_abi.SwigluBwdArgs)
+_pack_layer_norm = _abi.packer(_abi.LayerNormArgs)
+_pack_layer_norm_bwd = _abi.packer(_abi.LayerNormBwdArgs)
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -118,6 +120,95 @@ def ln_mod_bwd(x, dy, scale, mean, rstd, eps: float = 1e-6, dres=None, out=None)
         _rows(dres, "dres")
     _abi.call("fa_ln_mod_bwd", _pack_ln_bwd(*_ln_bwd_args(x, dy, scale, mean, rstd, eps, dres, dx)), _stream(x))
     return dx
+
+
+def _norm_rows(t: torch.Tensor, like: Optional[torch.Tensor], name: str) -> torch.Tensor:
+    """A 2-D row view [N, C] with unit column stride, of like's shape, dtype
+    and device when given."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or not t.is_cuda:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{name} must be a 2-D device tensor with contiguous rows")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
+                               f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
+    return t
+
+
+def _norm_vec(t: torch.Tensor, n: int, dtype, dev, name: str) -> torch.Tensor:
+    if t.shape != (n,) or not t.is_contiguous() or t.dtype != dtype or t.device != dev:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{name} must be a contiguous [{n}] {dtype} on {dev}")
+    return t
+
+
+def layer_norm_fwd(x, weight, bias=None, eps: float = 1e-5, out=None):
+    """Layer norm over the rows of x [N, C] with a learned weight [C] and
+    optional bias [C] (both bf16 or both f32, whatever x is): returns
+    (y, mean, rstd), the f32 row statistics as layer_norm_bwd needs them."""
+    x = _norm_rows(x, None, "x")
+    N, C = x.shape
+    _norm_vec(weight, C, weight.dtype, x.device, "weight")
+    if bias is not None:
+        _norm_vec(bias, C, weight.dtype, x.device, "bias")
+    y = torch.empty((N, C), dtype=x.dtype, device=x.device) if out is None else _norm_rows(out, x, "out")
+    mean, rstd = torch.empty((2, N), dtype=torch.float32, device=x.device).unbind()
+    a = _pack_layer_norm(_dtype_code(x), _dtype_code(weight), N, C, _f32(eps), x.data_ptr(), x.stride(0),
+                         weight.data_ptr(), _ptr(bias), y.data_ptr(), y.stride(0), mean.data_ptr(), rstd.data_ptr())
+    _abi.call("fa_layer_norm_fwd", a, _stream(x))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(x, dy, weight, mean, rstd, dres=None, out=None, want_dweight: bool = True,
+                   want_dbias: bool = True):
+    """(dx, dweight, dbias) of layer_norm_fwd for the upstream gradient dy,
+    dx = dres + ... when given; the parameters' gradients are f32 [C], None
+    where not wanted."""
+    x = _norm_rows(x, None, "x")
+    N, C = x.shape
+    dev = x.device
+    dy = _norm_rows(dy, x, "dy")
+    _norm_vec(weight, C, weight.dtype, dev, "weight")
+    _norm_vec(mean, N, torch.float32, dev, "mean")
+    _norm_vec(rstd, N, torch.float32, dev, "rstd")
+    if dres is not None:
+        _norm_rows(dres, x, "dres")
+    dx = torch.empty((N, C), dtype=x.dtype, device=dev) if out is None else _norm_rows(out, x, "out")
+    dw = torch.empty(C, dtype=torch.float32, device=dev) if want_dweight else None
+    db = torch.empty(C, dtype=torch.float32, device=dev) if want_dbias else None
+    stream = _stream(x)
+    head = (_dtype_code(x), _dtype_code(weight), N, C, 0.0, x.data_ptr(), x.stride(0), weight.data_ptr(), 0, 0, 0,
+            mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dy.stride(0), _ptr(dres),
+            0 if dres is None else dres.stride(0), dx.data_ptr(), dx.stride(0), _ptr(dw), _ptr(db))
+    ws, size = None, 0
+    if want_dweight or want_dbias:
+        size = max(_abi.entry("fa_layer_norm_bwd_workspace_size", size=True)(_pack_layer_norm_bwd(*head, 0, 0)), 256)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _abi.call("fa_layer_norm_bwd", _pack_layer_norm_bwd(*head, _ptr(ws), size), stream)
+    return dx, dw, db
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        x2 = x.reshape(-1, x.shape[-1])
+        y, mean, rstd = layer_norm_fwd(x2, weight, bias, eps)
+        ctx.save_for_backward(x2, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, weight, mean, rstd = ctx.saved_tensors
+        wb = ctx.bias_dtype is not None and ctx.needs_input_grad[2]
+        dx, dw, db = layer_norm_bwd(x2, dy.reshape(x2.shape).contiguous(), weight, mean, rstd,
+                                    want_dweight=ctx.needs_input_grad[1], want_dbias=wb)
+        return (dx.view(dy.shape) if ctx.needs_input_grad[0] else None, None if dw is None else dw.to(weight.dtype),
+                None if db is None else db.to(ctx.bias_dtype), None)
+
+
+def layer_norm(x, weight, bias=None, eps: float = 1e-5):
+    """Differentiable layer norm over x's last dim with a learned weight and
+    bias (layer_norm_fwd and layer_norm_bwd); the gradients of the parameters
+    come in their own dtype."""
+    return _LayerNormFn.apply(x, weight, bias, eps)
 
 
 def gated_ln_mod_fwd(x, g, b, shift, scale, eps: float = 1e-6, out=None, sum_out=None, sum_copy=None):

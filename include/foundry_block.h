@@ -9,6 +9,8 @@
  *   gated residual + layer_norm_mod   throughput.rs:552-566
  *                                        fa_gated_ln_mod_fwd / fa_ln_mod_bwd_gate
  *   gated residual   throughput.rs:552-572   fa_gated_residual
+ *   layer norm with a trained weight and bias (no reference counterpart: its
+ *                    norms are frozen)      fa_layer_norm_fwd / fa_layer_norm_bwd
  *   MLP activation   (c4 block: tanh-GELU; the reference block's SwiGLU,
  *                    lib.rs:293-297, has no tanh-GELU counterpart)
  *                                        fa_gelu_fwd / fa_gelu_bwd
@@ -103,6 +105,56 @@ typedef struct fa_ln_mod_bwd_gate_args {
  * fa_ln_mod_bwd followed by fa_gated_residual (x NULL) on its dx.  gdx must
  * not overlap dx. */
 fa_status fa_ln_mod_bwd_gate(const fa_ln_mod_bwd_gate_args *args, void *stream);
+
+typedef struct fa_layer_norm_args {
+    int32_t dtype;        /* fa_dtype of x, y (and dy, dres, dx)                 */
+    int32_t param_dtype;  /* fa_dtype of weight and bias                         */
+    int32_t rows, cols;   /* N >= 0; 1 <= C <= FA_LAYER_NORM_MAX_COLS            */
+    float eps;            /* > 0                                                 */
+    const void *x;        /* [N, C]                                              */
+    int64_t ldx;
+    const void *weight;   /* [C]                                                 */
+    const void *bias;     /* [C] or NULL (no bias)                               */
+    void *y;              /* [N, C] output (fwd)                                 */
+    int64_t ldy;
+    float *mean, *rstd;   /* [N] f32: written by fwd when non-NULL (rstd =
+                             1/sqrt(var + eps)); required by bwd                 */
+} fa_layer_norm_args;
+
+#define FA_LAYER_NORM_MAX_COLS 32768
+
+/* y = (x - mean) * rstd * weight + bias per row, mean and (biased) variance in
+ * f32.  Unlike the other row views of this header, any C and any row stride
+ * >= C will do, and rows and vectors need only their element's alignment.
+ * y may alias x element for element.  No reference counterpart: the
+ * reference's layer norms (lib.rs:60-71) have no learned weight. */
+fa_status fa_layer_norm_fwd(const fa_layer_norm_args *args, void *stream);
+
+typedef struct fa_layer_norm_bwd_args {
+    fa_layer_norm_args fwd; /* x, weight, mean, rstd as in the forward; bias, y,
+                             eps unused                                          */
+    const void *dy;       /* [N, C] gradient of y                                */
+    int64_t lddy;
+    const void *dres;     /* [N, C] or NULL: added to dx (a residual's gradient) */
+    int64_t ldres;
+    void *dx;             /* [N, C] output                                       */
+    int64_t lddx;
+    float *dweight;       /* [C] f32 output or NULL: sum over rows of dy * n     */
+    float *dbias;         /* [C] f32 output or NULL: sum over rows of dy         */
+    void *workspace;      /* device scratch, 256-byte aligned; unused (may be
+                             NULL) where dweight and dbias both are NULL         */
+    size_t workspace_bytes;
+} fa_layer_norm_bwd_args;
+
+/* Scratch bytes of fa_layer_norm_bwd's parameter gradients on the current
+ * device (0 for invalid sizes). */
+size_t fa_layer_norm_bwd_workspace_size(const fa_layer_norm_bwd_args *args);
+
+/* dx = dres + rstd * (g - mean(g) - n * mean(g * n)), n = (x - mean) * rstd,
+ * g = dy * weight, and the parameters' gradients.  Deterministic: the same
+ * bits on every call.  With no rows dweight and dbias are zero.  dx may alias
+ * dy, x or dres element for element. */
+fa_status fa_layer_norm_bwd(const fa_layer_norm_bwd_args *args, void *stream);
 
 typedef struct fa_rows_args {
     int32_t dtype;        /* fa_dtype of every view                              */
