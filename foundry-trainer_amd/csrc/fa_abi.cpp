@@ -299,10 +299,12 @@ size_t fwd_workspace(int32_t dtype, int32_t B, int32_t S, int32_t H, int32_t D) 
 namespace fa {
 hipError_t prepare_fwd_kernels();
 hipError_t prepare_bwd_kernels();
+hipError_t prepare_muon_kernels();
 hipError_t prepare_attn_kernels() {
     hipError_t e = prepare_fwd_kernels();
     if (e != hipSuccess) return e;
-    return prepare_bwd_kernels();
+    if ((e = prepare_bwd_kernels()) != hipSuccess) return e;
+    return prepare_muon_kernels();
 }
 }  // namespace fa
 
@@ -1363,6 +1365,122 @@ fa_status fa_adamw_step_many(const fa_adamw_args *args, int32_t count, void *str
         const hipError_t e = fa::launch_adamw_many(p, args[0].dtype, static_cast<hipStream_t>(stream));
         if (e != hipSuccess) return hip_fail(e, "adamw launch");
     }
+    return ok();
+}
+
+}  // extern "C"
+
+namespace {
+fa_status check_muon(const fa_muon_args *a) {
+    if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F32) return fail(FA_ERR_INVALID_ARG, "unknown dtype %d", a->dtype);
+    if (a->count < 1 || a->rows < 1 || a->cols < 1)
+        return fail(FA_ERR_INVALID_ARG, "count, rows and cols must be >= 1 (got %d, %d, %d)", a->count, a->rows, a->cols);
+    if (std::min(a->rows, a->cols) > FA_MUON_MAX_RANK || std::max(a->rows, a->cols) > (1 << 30))
+        return fail(FA_ERR_UNSUPPORTED, "%d x %d matrices: this build implements min(rows, cols) <= %d, max <= 2^30",
+                    a->rows, a->cols, FA_MUON_MAX_RANK);
+    if (!a->param || !a->grad || !a->momentum || !aligned(a->param, dtype_bytes(a->dtype)) || !aligned(a->grad, 4) ||
+        !aligned(a->momentum, 4))
+        return fail(FA_ERR_INVALID_ARG, "param/grad/momentum is NULL or misaligned");
+    if (!(a->lr >= 0.0) || !isfinite(a->lr) || !(a->beta >= 0.0 && a->beta < 1.0) || !(a->weight_decay >= 0.0) ||
+        !(a->lr * a->weight_decay <= 1.0) || !(a->eps > 0.0) || !isfinite(a->eps))
+        return fail(FA_ERR_INVALID_ARG, "need finite lr >= 0, 0 <= beta < 1, 0 <= lr * weight_decay <= 1, finite eps > 0");
+    if (!isfinite(a->scale) || !isfinite(a->a) || !isfinite(a->b) || !isfinite(a->c))
+        return fail(FA_ERR_INVALID_ARG, "scale and the coefficients must be finite");
+    if (a->steps < 0 || a->steps > FA_MUON_MAX_STEPS)
+        return fail(FA_ERR_INVALID_ARG, "steps %d not in 0..%d", a->steps, FA_MUON_MAX_STEPS);
+    return FA_OK;
+}
+
+fa_status check_muon_many(const fa_muon_args *args, int32_t count) {
+    if (!args || count < 1) return fail(FA_ERR_INVALID_ARG, "args is NULL or count < 1");
+    for (int32_t i = 0; i < count; ++i) {
+        FA_TRY(check_muon(&args[i]));
+        const fa_muon_args &a = args[i], &z = args[0];
+        if (a.dtype != z.dtype || a.lr != z.lr || a.beta != z.beta || a.weight_decay != z.weight_decay ||
+            a.eps != z.eps || a.a != z.a || a.b != z.b || a.c != z.c || a.steps != z.steps ||
+            (a.nesterov != 0) != (z.nesterov != 0))
+            return fail(FA_ERR_INVALID_ARG, "tensor %d: all but its sizes and scale must match tensor 0", i);
+    }
+    return FA_OK;
+}
+
+// Calls f on the step's tensors in launch sets of up to kMuonMany, those of one
+// number of row blocks together; ends with f's first false.
+template <typename F>
+bool muon_sets(const fa_muon_args *args, int32_t count, F f) {
+    for (int rb = 1; rb <= (FA_MUON_MAX_RANK + 15) / 16; ++rb) {
+        fa::MuonMany p{};
+        auto flush = [&] {
+            const bool fine = p.items == 0 || f(p);
+            p.items = 0;
+            return fine;
+        };
+        p.beta = (float)args[0].beta;
+        p.keep = (float)(1.0 - args[0].lr * args[0].weight_decay);
+        p.eps = args[0].eps;
+        p.a = args[0].a;
+        p.b = args[0].b;
+        p.c = args[0].c;
+        p.steps = args[0].steps;
+        p.nesterov = args[0].nesterov != 0;
+        for (int32_t i = 0; i < count; ++i) {
+            const fa_muon_args &a = args[i];
+            if (fa::muon_row_blocks(a.rows, a.cols) != rb) continue;
+            const int k = p.items++;
+            p.param[k] = a.param;
+            p.grad[k] = a.grad;
+            p.m[k] = a.momentum;
+            p.count[k] = a.count;
+            p.wide[k] = a.rows <= a.cols;
+            p.r[k] = std::min(a.rows, a.cols);
+            p.n[k] = std::max(a.rows, a.cols);
+            p.rate[k] = (float)(a.lr * a.scale);
+            if (p.items == fa::kMuonMany && !flush()) return false;
+        }
+        if (!flush()) return false;
+    }
+    return true;
+}
+
+// 0: a tensor has too many matrices for one launch
+size_t muon_workspace(const fa_muon_args *args, int32_t count) {
+    size_t most = 0;
+    const bool fine = muon_sets(args, count, [&](fa::MuonMany &p) {
+        const size_t n = fa::muon_workspace_bytes(p);
+        most = std::max(most, n);
+        return n > 0;
+    });
+    return fine ? most : 0;
+}
+}  // namespace
+
+extern "C" {
+
+size_t fa_muon_step_many_workspace_size(const fa_muon_args *args, int32_t count) {
+    if (!args || count < 1) return 0;
+    for (int32_t i = 0; i < count; ++i) {
+        const fa_muon_args &a = args[i];
+        if (a.count < 1 || a.rows < 1 || a.cols < 1 || std::min(a.rows, a.cols) > FA_MUON_MAX_RANK ||
+            std::max(a.rows, a.cols) > (1 << 30))
+            return 0;
+    }
+    return muon_workspace(args, count);
+}
+
+fa_status fa_muon_step_many(const fa_muon_args *args, int32_t count, void *workspace, size_t workspace_bytes,
+                            void *stream) {
+    FA_TRY(check_muon_many(args, count));
+    const size_t need = muon_workspace(args, count);
+    if (!need) return fail(FA_ERR_UNSUPPORTED, "too many matrices in a tensor (or set of tensors) for one launch");
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+        return fail(FA_ERR_INVALID_ARG, "workspace is NULL, not 256-byte aligned, or smaller than %zu bytes", need);
+    FA_TRY(init_current());
+    hipError_t e = hipSuccess;
+    muon_sets(args, count, [&](fa::MuonMany &p) {
+        e = fa::launch_muon_many(p, args[0].dtype, workspace, static_cast<hipStream_t>(stream));
+        return e == hipSuccess;
+    });
+    if (e != hipSuccess) return hip_fail(e, "muon launch");
     return ok();
 }
 

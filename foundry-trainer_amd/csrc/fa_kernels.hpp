@@ -267,6 +267,33 @@ struct AdamwMany {
 };
 hipError_t launch_adamw_many(AdamwMany p, int dtype, hipStream_t s);
 
+// Up to kMuonMany tensors of `count` matrices each, min(rows, cols) = r <=
+// kMuonMaxRank, n the other side, of one step (muon.hip).  What lies behind
+// `steps` is filled by the launcher.
+constexpr int kMuonMany = 32, kMuonMaxRank = 64;
+struct MuonMany {
+    void *param[kMuonMany];
+    const float *grad[kMuonMany];
+    float *m[kMuonMany];
+    int count[kMuonMany], r[kMuonMany], n[kMuonMany];
+    bool wide[kMuonMany];     // rows = r: rows contiguous along n; else columns are
+    float rate[kMuonMany];    // lr * scale
+    int items;
+    float beta, keep;         // keep = 1 - lr * weight_decay
+    double eps, a, b, c;
+    int nesterov, steps;
+    int chunk[kMuonMany], chunks[kMuonMany], block0[kMuonMany + 1], matrix0[kMuonMany + 1];
+    int64_t gram0[kMuonMany]; // first f64 of the tensor's Gram parts
+    size_t turn_at, expo_at;
+    double *gram;  // per matrix and chunk: Gram part
+    float *turn;   // per matrix: T
+    int *expo;     // per matrix: power of two that scales u
+};
+// Row blocks of 16 that a matrix takes; the tensors of a launch should agree in it.
+int muon_row_blocks(int rows, int cols);
+size_t muon_workspace_bytes(MuonMany &p);  // 0: too many for one launch
+hipError_t launch_muon_many(MuonMany &p, int dtype, void *work, hipStream_t s);
+
 }  // namespace fa
 
 namespace fa {

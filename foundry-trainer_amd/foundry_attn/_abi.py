@@ -36,6 +36,7 @@ EXPORTED = [
     "fa_lora_grad_many", "fa_lora_grad_many_workspace_size",
     "fa_gated_ln_mod_fwd", "fa_ln_mod_bwd_gate", "fa_gemm_bf16",
     "fa_layer_norm_fwd", "fa_layer_norm_bwd", "fa_layer_norm_bwd_workspace_size",
+    "fa_muon_step_many", "fa_muon_step_many_workspace_size",
 ]
 
 
@@ -209,6 +210,19 @@ class AdamwArgs(ctypes.Structure):
     ]
 
 
+FA_MUON_MAX_RANK, FA_MUON_MAX_STEPS = 64, 10
+
+
+class MuonArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("count", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
+        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("momentum", ctypes.c_void_p),
+        ("lr", ctypes.c_double), ("beta", ctypes.c_double), ("weight_decay", ctypes.c_double),
+        ("eps", ctypes.c_double), ("scale", ctypes.c_double), ("a", ctypes.c_double), ("b", ctypes.c_double),
+        ("c", ctypes.c_double), ("steps", ctypes.c_int32), ("nesterov", ctypes.c_int32),
+    ]
+
+
 class Copy2dArgs(ctypes.Structure):
     _fields_ = [
         ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32),
@@ -261,6 +275,11 @@ def lib() -> ctypes.CDLL:
     L.fa_qk_prologue_bwd_multi.argtypes = [ctypes.POINTER(QkPrologueBwdArgs), ctypes.c_int32, ctypes.c_void_p]
     L.fa_adamw_step_many.restype = ctypes.c_int
     L.fa_adamw_step_many.argtypes = [ctypes.POINTER(AdamwArgs), ctypes.c_int32, ctypes.c_void_p]
+    L.fa_muon_step_many.restype = ctypes.c_int
+    L.fa_muon_step_many.argtypes = [ctypes.POINTER(MuonArgs), ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
+                                    ctypes.c_void_p]
+    L.fa_muon_step_many_workspace_size.restype = ctypes.c_size_t
+    L.fa_muon_step_many_workspace_size.argtypes = [ctypes.POINTER(MuonArgs), ctypes.c_int32]
     L.fa_copy2d_many.restype = ctypes.c_int
     L.fa_copy2d_many.argtypes = [ctypes.POINTER(Copy2dArgs), ctypes.c_int32, ctypes.c_void_p]
     L.fa_attn_bwd_phase.restype = ctypes.c_int

@@ -63,6 +63,7 @@ _pack_swiglu = _abi.packer(_abi.SwigluArgs)
 _pack_swiglu_bwd = _abi.packer(_abi.SwigluBwdArgs)
 _pack_layer_norm = _abi.packer(_abi.LayerNormArgs)
 _pack_layer_norm_bwd = _abi.packer(_abi.LayerNormBwdArgs)
+_pack_muon = _abi.packer(_abi.MuonArgs)
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -374,6 +375,59 @@ def adamw_step_many(items, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps:
                                 v=_ptr(v), lr=float(lr), beta1=float(betas[0]), beta2=float(betas[1]),
                                 eps=float(eps), step=int(step))
     check(lib().fa_adamw_step_many(arr, len(items), _stream(items[0][0])))
+
+
+MUON_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: float = 0.0, steps: int = 5,
+                   nesterov: bool = True, eps: float = 1e-7, coeffs=MUON_COEFFS, scale: Optional[float] = None):
+    """One optimiser step with orthogonalised updates over (param, grad,
+    momentum) triples, in place on param and momentum (fa_muon_step_many):
+      m = beta m + g;  u = g + beta m (nesterov) or m
+      X = u / (|u| + eps);  `steps` times X = a X + (b X X^T + c (X X^T)^2) X
+      p = p (1 - lr weight_decay) - lr scale X
+    param is [rows, cols] or [n, rows, cols] (n matrices, each by itself, e.g. a
+    pool's factors), bf16 or f32, min(rows, cols) <= 64; grad and momentum are
+    f32 of its shape; all contiguous, the params of one dtype on one device.
+    scale: default sqrt(max(1, rows / cols)) of each."""
+    items = list(items)
+    if not items:
+        return
+    first = items[0][0]
+    dev, code = first.device, _dtype_code(first)
+    if not first.is_cuda:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "params must be device tensors")
+    ca, cb, cc = (float(v) for v in coeffs)
+    packed, count = [], 0
+    for p, g, m in items:
+        if p.dim() not in (2, 3) or not p.is_contiguous() or p.dtype != first.dtype or p.device != dev:
+            raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
+                                   f"params must be contiguous 2-D or 3-D {first.dtype} tensors on {dev}")
+        for name, t in (("grad", g), ("momentum", m)):
+            if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev:
+                raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
+                                       f"{name} must be contiguous float32 {list(p.shape)} on {dev}")
+        if p.dim() == 3 and p.shape[0] == 0:
+            continue
+        rows, cols = p.shape[-2:]
+        sc = math.sqrt(max(1.0, rows / max(cols, 1))) if scale is None else float(scale)
+        packed.append(_pack_muon(code, p.shape[0] if p.dim() == 3 else 1, rows, cols, p.data_ptr(), g.data_ptr(),
+                                 m.data_ptr(), float(lr), float(beta), float(weight_decay), float(eps), sc, ca, cb,
+                                 cc, int(steps), int(bool(nesterov))))
+        count += 1
+    if not count:
+        return
+    arr, stream = b"".join(packed), _stream(first)
+    need = max(_abi.entry("fa_muon_step_many_workspace_size", ctypes.c_int32, size=True)(arr, count), 256)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    check(_abi.entry("fa_muon_step_many", ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p)(
+        arr, count, ws.data_ptr(), need, stream))
+
+
+def muon_step(param, grad, momentum, **kw):
+    """muon_step_many of one tensor."""
+    muon_step_many([(param, grad, momentum)], **kw)
 
 
 def _set_mod(old, parts):

@@ -19,6 +19,8 @@
  *                                        fa_swiglu_fwd / fa_swiglu_bwd
  *   modulation input silu(temb)  throughput.rs:297-324     fa_silu
  *   adamw_step       lib.rs:477-510      fa_adamw_step, fa_adamw_step_many
+ *   orthogonalised step of low-rank factors (no reference counterpart)
+ *                                        fa_muon_step_many
  *   MLP linear + activation  linear_scaled's base product lib.rs:270-287
  *                    at throughput.rs:254-256, fused with the GELU that
  *                    follows W1 or the GELU gradient after W2's dX
@@ -243,6 +245,46 @@ fa_status fa_adamw_step(const fa_adamw_args *args, void *stream);
  * reference steps each parameter in turn (lib.rs:477-510 inside the loop of
  * throughput.rs:787-803). */
 fa_status fa_adamw_step_many(const fa_adamw_args *args, int32_t count, void *stream);
+
+typedef struct fa_muon_args {
+    int32_t dtype;        /* fa_dtype of param                                   */
+    int32_t count;        /* matrices, one after another, >= 1                   */
+    int32_t rows, cols;   /* of each: min(rows, cols) in 1..FA_MUON_MAX_RANK,
+                             max(rows, cols) <= 2^30                             */
+    void *param;          /* [count, rows, cols] contiguous, updated in place    */
+    const float *grad;    /* [count, rows, cols] f32                             */
+    float *momentum;      /* [count, rows, cols] f32, updated in place (zero at
+                             the first step)                                     */
+    double lr;            /* >= 0                                                */
+    double beta;          /* momentum, 0 <= beta < 1                             */
+    double weight_decay;  /* decoupled, >= 0, lr * weight_decay <= 1             */
+    double eps;           /* > 0, added to the Frobenius norm                    */
+    double scale;         /* of the orthogonalised update, e.g.
+                             sqrt(max(1, rows / cols)); finite                   */
+    double a, b, c;       /* coefficients of one product, finite                 */
+    int32_t steps;        /* products, 0..FA_MUON_MAX_STEPS                      */
+    int32_t nesterov;     /* 0 or 1                                              */
+} fa_muon_args;
+
+#define FA_MUON_MAX_RANK 64
+#define FA_MUON_MAX_STEPS 10
+
+/* One optimiser step with orthogonalised updates over `count` tensors of
+ * matrices (LoRA factors), each matrix by itself:
+ *   m = beta m + g;  u = nesterov ? g + beta m : m
+ *   X = u / (|u|_F + eps);  `steps` times X = a X + (b X X^T + c (X X^T)^2) X
+ *   p = p (1 - lr weight_decay) - lr scale X
+ * (X transposed where rows > cols).  The Gram matrix and the iteration are f64,
+ * the rest is f32, p is rounded once.  A matrix of zeros keeps a zero update;
+ * one with a NaN or infinity gets NaN all over.  All tensors share dtype, lr,
+ * beta, weight_decay, eps, a, b, c, steps and nesterov.  Matrices must not
+ * overlap.  Each gets the same bits whatever else the call holds.  One
+ * workspace of fa_muon_step_many_workspace_size bytes (0 for invalid
+ * arguments), 256-byte aligned.  No reference counterpart (its optimiser is
+ * AdamW, lib.rs:477-510). */
+size_t fa_muon_step_many_workspace_size(const fa_muon_args *args, int32_t count);
+fa_status fa_muon_step_many(const fa_muon_args *args, int32_t count, void *workspace, size_t workspace_bytes,
+                            void *stream);
 
 typedef struct fa_copy2d_args {
     int32_t dtype;            /* fa_dtype of src and dst                         */
