@@ -300,11 +300,13 @@ namespace fa {
 hipError_t prepare_fwd_kernels();
 hipError_t prepare_bwd_kernels();
 hipError_t prepare_muon_kernels();
+hipError_t prepare_pool_kernels();
 hipError_t prepare_attn_kernels() {
     hipError_t e = prepare_fwd_kernels();
     if (e != hipSuccess) return e;
     if ((e = prepare_bwd_kernels()) != hipSuccess) return e;
-    return prepare_muon_kernels();
+    if ((e = prepare_muon_kernels()) != hipSuccess) return e;
+    return prepare_pool_kernels();
 }
 }  // namespace fa
 
@@ -1481,6 +1483,130 @@ fa_status fa_muon_step_many(const fa_muon_args *args, int32_t count, void *works
         return e == hipSuccess;
     });
     if (e != hipSuccess) return hip_fail(e, "muon launch");
+    return ok();
+}
+
+}  // extern "C"
+
+namespace {
+static_assert(FA_LORA_POOL_MAX_ADAPTERS == fa::kPoolMaxAdapters);
+constexpr int32_t kPoolMaxTokens = 1 << 28, kPoolMaxFeatures = 1 << 22;
+
+bool pool_sizes(int32_t tokens, int32_t adapters) {
+    return tokens >= 0 && tokens <= kPoolMaxTokens && adapters >= 1 && adapters <= FA_LORA_POOL_MAX_ADAPTERS;
+}
+bool pool_sizes(const fa_lora_pool_args *a) {
+    return pool_sizes(a->tokens, a->adapters) && a->in_features >= 1 && a->in_features <= kPoolMaxFeatures &&
+           a->out_features >= 1 && a->out_features <= kPoolMaxFeatures && a->rank >= 1 && a->rank <= 64;
+}
+
+fa::PoolCall pool_call(const fa_lora_pool_args *a) {
+    fa::PoolCall c{};
+    c.plan = static_cast<const int *>(a->plan);
+    c.scale = a->scale;
+    c.x = a->x;
+    c.ldx = a->ldx;
+    c.a = a->a;
+    c.b = a->b;
+    c.u = a->u;
+    c.y = a->y;
+    c.ldy = a->ldy;
+    c.work = a->workspace;
+    c.T = a->tokens;
+    c.L = a->adapters;
+    c.K = a->in_features;
+    c.M = a->out_features;
+    c.r = a->rank;
+    return c;
+}
+
+fa_status check_pool_workspace(const fa_lora_pool_args *a, size_t need) {
+    if (need && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
+        return fail(FA_ERR_INVALID_ARG, "workspace is NULL, not 256-byte aligned, or smaller than %zu bytes", need);
+    return FA_OK;
+}
+
+fa_status check_pool(const fa_lora_pool_args *a) {
+    if (a->dtype != FA_DTYPE_BF16 && a->dtype != FA_DTYPE_F32) return fail(FA_ERR_INVALID_ARG, "unknown dtype %d", a->dtype);
+    if (!pool_sizes(a))
+        return fail(FA_ERR_INVALID_ARG,
+                    "tokens %d, features %d and %d, rank %d, adapters %d: need tokens 0..2^28, features 1..2^22, rank "
+                    "1..64, adapters 1..%d",
+                    a->tokens, a->in_features, a->out_features, a->rank, a->adapters, FA_LORA_POOL_MAX_ADAPTERS);
+    const size_t eb = dtype_bytes(a->dtype);
+    FA_TRY(check_any_view("x", a->x, a->ldx, a->tokens, a->in_features, a->dtype));
+    if (!a->a || !aligned(a->a, eb) || !a->b || !aligned(a->b, eb))
+        return fail(FA_ERR_INVALID_ARG, "a or b is NULL or misaligned");
+    if (!a->scale || !aligned(a->scale, 4)) return fail(FA_ERR_INVALID_ARG, "scale is NULL or misaligned");
+    if (!a->plan || !aligned(a->plan, 16) || a->plan_bytes < fa::pool_plan_bytes(a->tokens, a->adapters))
+        return fail(FA_ERR_INVALID_ARG, "plan is NULL, not 16-byte aligned, or smaller than %zu bytes",
+                    fa::pool_plan_bytes(a->tokens, a->adapters));
+    if ((!a->u && a->tokens > 0) || !aligned(a->u, 4)) return fail(FA_ERR_INVALID_ARG, "u is NULL or misaligned");
+    return FA_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t fa_lora_pool_plan_size(int32_t tokens, int32_t adapters) {
+    return pool_sizes(tokens, adapters) ? fa::pool_plan_bytes(tokens, adapters) : 0;
+}
+
+fa_status fa_lora_pool_plan(const int32_t *index, int32_t tokens, int32_t adapters, void *plan, size_t plan_bytes,
+                            void *stream) {
+    if (!pool_sizes(tokens, adapters))
+        return fail(FA_ERR_INVALID_ARG, "tokens %d, adapters %d: need tokens 0..2^28, adapters 1..%d", tokens, adapters,
+                    FA_LORA_POOL_MAX_ADAPTERS);
+    if ((!index && tokens > 0) || !aligned(index, 4)) return fail(FA_ERR_INVALID_ARG, "index is NULL or misaligned");
+    if (!plan || !aligned(plan, 16) || plan_bytes < fa::pool_plan_bytes(tokens, adapters))
+        return fail(FA_ERR_INVALID_ARG, "plan is NULL, not 16-byte aligned, or smaller than %zu bytes",
+                    fa::pool_plan_bytes(tokens, adapters));
+    FA_TRY(init_current());
+    const hipError_t e = fa::launch_pool_plan(index, tokens, adapters, static_cast<int *>(plan),
+                                              static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "pool plan launch");
+    return ok();
+}
+
+size_t fa_lora_pool_fwd_workspace_size(const fa_lora_pool_args *a) {
+    return a && pool_sizes(a) ? fa::pool_fwd_workspace_bytes(pool_call(a)) : 0;
+}
+
+fa_status fa_lora_pool_fwd(const fa_lora_pool_args *a, void *stream) {
+    if (!a) return fail(FA_ERR_INVALID_ARG, "args is NULL");
+    FA_TRY(check_pool(a));
+    FA_TRY(check_any_view("y", a->y, a->ldy, a->tokens, a->out_features, a->dtype));
+    const fa::PoolCall c = pool_call(a);
+    FA_TRY(check_pool_workspace(a, fa::pool_fwd_workspace_bytes(c)));
+    FA_TRY(init_current());
+    const hipError_t e = fa::launch_pool_fwd(c, a->dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "pool forward launch");
+    return ok();
+}
+
+size_t fa_lora_pool_bwd_workspace_size(const fa_lora_pool_bwd_args *a) {
+    return a && pool_sizes(&a->fwd) ? fa::pool_bwd_workspace_bytes(pool_call(&a->fwd)) : 0;
+}
+
+fa_status fa_lora_pool_bwd(const fa_lora_pool_bwd_args *a, void *stream) {
+    if (!a) return fail(FA_ERR_INVALID_ARG, "args is NULL");
+    const fa_lora_pool_args *f = &a->fwd;
+    FA_TRY(check_pool(f));
+    FA_TRY(check_any_view("dy", a->dy, a->ldy, f->tokens, f->out_features, f->dtype));
+    if (a->dx) FA_TRY(check_any_view("dx", a->dx, a->ldx, f->tokens, f->in_features, f->dtype));
+    if ((a->da == nullptr) != (a->db == nullptr) || !aligned(a->da, 4) || !aligned(a->db, 4))
+        return fail(FA_ERR_INVALID_ARG, "da and db must both be given or both NULL, 4-byte aligned");
+    fa::PoolCall c = pool_call(f);
+    FA_TRY(check_pool_workspace(f, fa::pool_bwd_workspace_bytes(c)));
+    c.dy = a->dy;
+    c.lddy = a->ldy;
+    c.da = a->da;
+    c.db = a->db;
+    c.dx = a->dx;
+    c.lddx = a->ldx;
+    FA_TRY(init_current());
+    const hipError_t e = fa::launch_pool_bwd(c, f->dtype, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "pool backward launch");
     return ok();
 }
 

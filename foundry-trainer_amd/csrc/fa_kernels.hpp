@@ -148,6 +148,41 @@ struct LoraGradItem {
 size_t lora_grad_many_workspace_bytes(const LoraGradItem *items, int count);
 hipError_t launch_lora_grad_many_bf16(const LoraGradItem *items, int count, void *work, hipStream_t st);
 
+// A pool of adapters (lora_pool.hip).  One kernel's view of a call: `low` is u
+// or v, [splits][T][r] f32.
+constexpr int kPoolMaxAdapters = 2048;
+struct PoolParams {
+    const int *plan;
+    const float *scale;  // [L]
+    const void *x;       // wide rows read
+    int64_t ldx;
+    const void *factor;  // [L, r, wide] or [L, wide, r]
+    float *low, *low_out;
+    void *y;             // wide rows updated
+    int64_t ldy;
+    int T, L, r, wide, splits;
+};
+struct PoolGradParams {
+    float *out, *part;   // [L] and [slots] gradients of r * wide elements
+    int blocks, slots, transpose;
+};
+struct PoolCall {
+    const int *plan;
+    const float *scale;
+    const void *x, *a, *b, *dy;
+    void *y, *dx;
+    float *u, *da, *db;
+    int64_t ldx, ldy, lddy, lddx;
+    void *work;
+    int T, L, K, M, r;
+};
+size_t pool_plan_bytes(int T, int L);
+hipError_t launch_pool_plan(const int *index, int T, int L, int *plan, hipStream_t s);
+size_t pool_fwd_workspace_bytes(const PoolCall &c);
+size_t pool_bwd_workspace_bytes(const PoolCall &c);
+hipError_t launch_pool_fwd(const PoolCall &c, int dtype, hipStream_t s);
+hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s);
+
 // LayerNorm-modulation over [N, C] rows (C % 8 == 0, C <= 4096).
 struct LnModParams {
     const void *x;

@@ -1,0 +1,756 @@
+// A pool of LoRA adapters beside one shared projection.  Token t belongs to
+// adapter i = index[t], or to none where index[t] is outside 0..L-1:
+//   u[t]  = A_i x[t]             y[t]  += s_i B_i u[t]
+//   v[t]  = B_i^T dy[t]          dx[t] += s_i A_i^T v[t]
+//   dA_i  = s_i sum_t v[t] x[t]^T     dB_i = s_i sum_t dy[t] u[t]^T
+// with A [L, r, K], B [L, M, r].
+//
+// The plan (pool_plan_kernel) sorts the tokens by adapter, stably, and cuts each
+// adapter's tokens into row tiles of 64 and gradient chunks of 256; all other
+// kernels run on a grid of the most tiles there can be and leave at once where
+// there is none, so nothing of the index has to come back to the host.
+//   pool_down   64 rows x a range of the wide axis: u or v, f32, over `splits`
+//               ranges that the reader adds in order
+//   pool_up     64 rows x 256 columns: y or dx
+//   pool_grad   a chunk x 512 (f32: 256) columns of dA or dB: straight to the
+//               result where the adapter has one chunk, else a partial sum
+//   pool_reduce the partial sums in order, and zeros for adapters without tokens
+// u and v are f32 between the kernels.  bf16 products (v_mfma_f32_16x16x32) take
+// them as sums of bf16 terms, high part first: two terms (2^-17) where the result
+// is rounded to bf16, three (2^-25) where it stays f32.  f32 products are
+// v_mfma_f32_16x16x4.  No atomics: the same bits every time.
+#include <algorithm>
+#include <type_traits>
+
+#include "fa_device.hpp"
+#include "fa_kernels.hpp"
+
+namespace fa {
+namespace {
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+constexpr int kRows = 64;     // of a row tile
+constexpr int kChunk = 256;   // rows of a gradient chunk
+constexpr int kPlanWaves = 16;
+
+// ---------------------------------------------------------------------------
+// the plan: int32 words
+// ---------------------------------------------------------------------------
+struct Tile {
+    int start, rows, adapter, slot;  // rows perm[start .. start + rows); adapter -1: none
+};
+struct PlanView {
+    int *head;    // tiles, chunks
+    int *perm;    // [T] tokens sorted by adapter, those without one last
+    int *count;   // [L] tokens of each adapter
+    int *slot0;   // [L] its first partial gradient; -1: none (at most one chunk)
+    Tile *tiles, *chunks;
+};
+__host__ __device__ inline int64_t most_tiles(int64_t T, int64_t L, int rows) {
+    return (T + rows - 1) / rows + (L + 1 < T ? L + 1 : T);
+}
+__host__ __device__ inline int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
+__host__ __device__ inline int64_t plan_words(int64_t T, int64_t L) {
+    return 4 + round4(T) + 2 * round4(L) + 4 * (most_tiles(T, L, kRows) + most_tiles(T, L, kChunk));
+}
+__host__ __device__ inline PlanView plan_view(int *p, int64_t T, int64_t L) {
+    PlanView v;
+    v.head = p;
+    v.perm = p + 4;
+    v.count = v.perm + round4(T);
+    v.slot0 = v.count + round4(L);
+    v.tiles = reinterpret_cast<Tile *>(v.slot0 + round4(L));
+    v.chunks = v.tiles + most_tiles(T, L, kRows);
+    return v;
+}
+
+// One workgroup.  Wave w holds the w-th sixteenth of the tokens; hist[w][a]
+// first counts its tokens of adapter a (a = L: none), then holds where in perm
+// they begin.
+__global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T, int L, int *plan) {
+    extern __shared__ int hist[];  // [kPlanWaves][L + 1], then [3][L + 2]: rows, tiles and chunks before adapter a
+    __shared__ int carry[kPlanWaves][4], total[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, A = L + 1;
+    int *rows0 = hist + kPlanWaves * A, *tiles0 = rows0 + L + 2, *chunks0 = tiles0 + L + 2;
+    const PlanView v = plan_view(plan, T, L);
+    for (int i = tid; i < kPlanWaves * A; i += 1024) hist[i] = 0;
+    __syncthreads();
+    const int64_t share = (((int64_t)T + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
+    const int64_t t0 = wave * share, t1 = std::min<int64_t>(T, t0 + share);
+    auto adapter_of = [&](int64_t t) {
+        const int a = t < t1 ? index[t] : -2;
+        return t >= t1 ? -1 : (a < 0 || a >= L ? L : a);
+    };
+    // f(adapter, its lanes) for each adapter among the wave's next 64 tokens
+    auto each = [&](int a, auto f) {
+        uint64_t left = __ballot(a >= 0);
+        while (left) {
+            const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
+            const uint64_t same = __ballot(a == cur);
+            f(cur, same);
+            left &= ~same;
+        }
+    };
+    for (int64_t t = t0; t < t1; t += 64)
+        each(adapter_of(t + lane), [&](int a, uint64_t same) {
+            hist[wave * A + a] += __popcll(same);  // every lane the same
+        });
+    __syncthreads();
+    // exclusive sums over adapters of rows, tiles, chunks and partial slots:
+    // thread i holds the E adapters from i * E on
+    const int E = (A + 1023) / 1024;
+    int own[4] = {0, 0, 0, 0};
+    auto add = [&](int a, int s[4]) {
+        int n = 0;
+        for (int w = 0; w < kPlanWaves; ++w) n += hist[w * A + a];
+        const int c = a < L ? (n + kChunk - 1) / kChunk : 0;
+        s[0] += n;
+        s[1] += (n + kRows - 1) / kRows;
+        s[2] += c;
+        s[3] += c > 1 ? c : 0;
+        return n;
+    };
+    for (int e = 0; e < E; ++e)
+        if (tid * E + e < A) add(tid * E + e, own);
+    int before[4];
+    for (int k = 0; k < 4; ++k) {
+        int s = own[k];
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(s, d, 64);
+            if (lane >= d) s += o;
+        }
+        if (lane == 63) carry[wave][k] = s;
+        before[k] = s - own[k];
+    }
+    __syncthreads();
+    for (int k = 0; k < 4; ++k)
+        for (int w = 0; w < wave; ++w) before[k] += carry[w][k];
+    for (int e = 0; e < E; ++e) {
+        const int a = tid * E + e;
+        if (a >= A) break;
+        rows0[a] = before[0];
+        tiles0[a] = before[1];
+        chunks0[a] = before[2];
+        const int slot0 = before[3];
+        const int n = add(a, before);
+        if (a < L) {
+            v.count[a] = n;
+            v.slot0[a] = before[3] > slot0 ? slot0 : -1;
+        }
+        if (a == L) {
+            rows0[A] = before[0];
+            tiles0[A] = before[1];
+            chunks0[A] = before[2];
+            for (int k = 0; k < 4; ++k) total[k] = before[k];
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        v.head[0] = total[1];
+        v.head[1] = total[2];
+        v.head[2] = T;
+        v.head[3] = L;
+    }
+    for (int a = tid; a < A; a += 1024) {
+        int at = rows0[a];
+        for (int w = 0; w < kPlanWaves; ++w) {
+            const int n = hist[w * A + a];
+            hist[w * A + a] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    for (int64_t t = t0; t < t1; t += 64)
+        each(adapter_of(t + lane), [&](int a, uint64_t same) {
+            const int at = hist[wave * A + a];
+            if (same >> lane & 1) v.perm[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)(t + lane);
+            hist[wave * A + a] = at + __popcll(same);
+        });
+    auto find = [&](const int *first, int i) {  // the adapter a with first[a] <= i < first[a + 1]
+        int lo = 0, hi = A - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (first[mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    for (int i = tid; i < total[1]; i += 1024) {
+        const int a = find(tiles0, i), k = i - tiles0[a], start = rows0[a] + k * kRows;
+        v.tiles[i] = Tile{start, std::min(kRows, rows0[a + 1] - start), a < L ? a : -1, 0};
+    }
+    for (int i = tid; i < total[2]; i += 1024) {
+        const int a = find(chunks0, i), k = i - chunks0[a], start = rows0[a] + k * kChunk;
+        v.chunks[i] = Tile{start, std::min(kChunk, rows0[a + 1] - start), a, chunks0[a + 1] - chunks0[a] > 1 ? k : -1};
+    }
+}
+
+// A tile of the plan as the kernels trust it: nothing of it leads outside the
+// call's tensors, whatever memory the plan was given.
+__device__ __forceinline__ bool tile_of(const PoolParams &p, bool chunk, int i, Tile &t) {
+    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    if (v.head[2] != p.T || v.head[3] != p.L) return false;
+    const int n = chunk ? v.head[1] : v.head[0];
+    if (i >= n) return false;
+    t = (chunk ? v.chunks : v.tiles)[i];
+    const int most = chunk ? kChunk : kRows;
+    return t.start >= 0 && t.rows > 0 && t.rows <= most && t.start <= p.T - t.rows && t.adapter < p.L;
+}
+// Token of row i of a tile; past its end the last one's (read, never written).
+__device__ __forceinline__ int token_of(const PoolParams &p, const Tile &t, int i) {
+    const int *perm = p.plan + 4;
+    const int row = perm[t.start + std::min(i, t.rows - 1)];
+    return (unsigned)row < (unsigned)p.T ? row : 0;
+}
+
+// ---------------------------------------------------------------------------
+// loads and operands
+// ---------------------------------------------------------------------------
+// 16 bytes from column c of a row of n elements; zero past its end.
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T *row, int64_t c, int64_t n) {
+    constexpr int E = 16 / sizeof(T);
+    if (c + E <= n) return *reinterpret_cast<const u32x4_any *>(row + c);
+    T v[E] = {};
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (c + j < n) v[j] = row[c + j];
+    u32x4 r;
+    __builtin_memcpy(&r, v, 16);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T *row, int64_t c, int64_t n, u32x4 w) {
+    constexpr int E = 16 / sizeof(T);
+    if (c + E <= n) {
+        *reinterpret_cast<u32x4_any *>(row + c) = w;
+        return;
+    }
+    T v[E];
+    __builtin_memcpy(v, &w, 16);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (c + j < n) row[c + j] = v[j];
+}
+__device__ __forceinline__ f32x4 load_f4(const float *base, int left) {
+    if (left >= 4) return *reinterpret_cast<const f32x4_any *>(base);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < left) v[j] = base[j];
+    return v;
+}
+__device__ __forceinline__ void store_f4(float *base, int left, f32x4 v) {
+    if (left >= 4) {
+        *reinterpret_cast<f32x4_any *>(base) = v;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < left) base[j] = v[j];
+}
+
+// acc += A B over the 16 bytes per lane of both: 8 bf16 (K = 32 with the four
+// lane groups) or 4 f32 (K = 16)
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 acc) {
+    if constexpr (sizeof(T) == 2) return mfma_16x16x32(as_bf16x8(a), as_bf16x8(b), acc);
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = mfma_16x16x4_f32(x[j], y[j], acc);
+    return acc;
+}
+
+// v as a sum of bf16 terms: term k rounds what the terms before it left.
+template <int TERMS>
+__device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TERMS]) {
+    float rest[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rest[j] = v[j];
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+        bf16x8 t;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            t[j] = f32_to_bf16(rest[j]);
+            rest[j] -= (float)t[j];
+        }
+        out[k] = as_u32x4(t);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// pool_down: u = A x (ROWMAJOR: the factor's rows run along the wide axis) or
+// v = B^T dy (B [wide][r])
+// ---------------------------------------------------------------------------
+// D[rank][token]: the factor is the A operand, the tokens' rows the B operand.
+// A wave takes every fourth 128-byte step of the range; a lane's 32 bytes of a
+// row are two operands.
+template <typename T, int RB, bool ROWMAJOR>
+__global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
+    constexpr int E = 16 / sizeof(T), STEP = 8 * E;
+    __shared__ f32x4 sum[4][RB][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    Tile t;
+    if (!tile_of(p, false, blockIdx.x, t)) return;
+    const int r = p.r, W = p.wide;
+    const int64_t part = (int64_t)blockIdx.y * p.T;
+    if (t.adapter < 0) {
+        for (int i = threadIdx.x; i < t.rows * r; i += 256)
+            p.low[(part + token_of(p, t, i / r)) * r + i % r] = 0.f;
+        return;
+    }
+    const int subs = (t.rows + 15) / 16;
+    const int64_t steps = ((int64_t)W + STEP - 1) / STEP;
+    const int64_t s0 = steps * blockIdx.y / gridDim.y, s1 = steps * (blockIdx.y + 1) / gridDim.y;
+    const T *rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = static_cast<const T *>(p.x) + token_of(p, t, 16 * i + x) * p.ldx;
+    const T *factor = static_cast<const T *>(p.factor) + (int64_t)t.adapter * r * W;
+    f32x4 acc[RB][4];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int64_t s = s0 + wave; s < s1; s += 4) {
+        const int64_t c = s * STEP + 2 * E * q;
+        u32x4 f[RB][2], d[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < subs) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) d[i][h] = load16(rows[i], c + E * h, W);
+            }
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            const int i = 16 * b + x;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (ROWMAJOR) {
+                    f[b][h] = i < r ? load16(factor + (int64_t)i * W, c + E * h, W) : u32x4{0, 0, 0, 0};
+                } else {
+                    T v[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const int64_t m = c + E * h + e;
+                        v[e] = i < r && m < W ? factor[m * r + i] : (T)0.f;
+                    }
+                    __builtin_memcpy(&f[b][h], v, 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < subs) {
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) acc[b][i] = mfma16<T>(f[b][h], d[i][h], acc[b][i]);
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[wave][b][i][lane] = acc[b][i];
+    __syncthreads();
+    // wave i stores rows 16 i .. + 16: ranks 16 b + 4 q .. + 4 of token x
+    if (16 * wave + x >= t.rows) return;
+    float *out = p.low + (part + token_of(p, t, 16 * wave + x)) * r;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        f32x4 v = sum[0][b][wave][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += sum[w][b][wave][lane];
+        store_f4(out + 16 * b + 4 * q, r - 16 * b - 4 * q, v);
+    }
+}
+
+// Ranks i .. i + 4 of a token's u or v: its `splits` parts in order.
+__device__ __forceinline__ f32x4 low_f4(const PoolParams &p, int token, int i) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s)
+        v += load_f4(p.low + ((int64_t)s * p.T + token) * p.r + i, p.r - i);
+    return v;
+}
+
+// ---------------------------------------------------------------------------
+// pool_up: y += s B u (ROWMAJOR: the factor's rows run along the rank) or
+// dx += s A^T v (A [r][wide])
+// ---------------------------------------------------------------------------
+// D[column][token]: a wave's step is 64 columns in four products; row 4 q + v of
+// product j is column 16 q + 4 j + v, so that a lane ends with 16 consecutive
+// columns of its token.
+template <typename T, int RB, bool ROWMAJOR>
+__global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
+    constexpr int E = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    Tile t;
+    if (!tile_of(p, false, blockIdx.x, t)) return;
+    const int r = p.r, W = p.wide;
+    const int subs = (t.rows + 15) / 16;
+    if (p.low_out && blockIdx.y == 0) {  // the parts' sum, for the backward
+        for (int i = threadIdx.x; i < t.rows * ((r + 3) / 4); i += 256) {
+            const int token = token_of(p, t, i / ((r + 3) / 4)), k = i % ((r + 3) / 4) * 4;
+            store_f4(p.low_out + (int64_t)token * r + k, r - k, low_f4(p, token, k));
+        }
+    }
+    if (t.adapter < 0) return;
+    const float scale = p.scale[t.adapter];
+    const T *factor = static_cast<const T *>(p.factor) + (int64_t)t.adapter * r * W;
+    // the tokens' operand: bf16 takes the high parts of 16 ranks in lane groups
+    // 0 and 1, what they leave in 2 and 3; f32 ranks 4 q .. + 4
+    u32x4 low[RB][4];
+    T *out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int token = token_of(p, t, 16 * i + x);
+        out[i] = static_cast<T *>(p.y) + token * p.ldy;
+        if (i < subs) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                if constexpr (sizeof(T) == 2) {
+                    const int k = 16 * b + 8 * (q & 1);
+                    const f32x4 a = low_f4(p, token, k), c = low_f4(p, token, k + 4);
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = a[j] * scale;
+                        v[4 + j] = c[j] * scale;
+                    }
+                    u32x4 terms[2];
+                    split_terms(v, terms);
+                    low[b][i] = q < 2 ? terms[0] : terms[1];
+                } else {
+                    low[b][i] = __builtin_bit_cast(u32x4, low_f4(p, token, 16 * b + 4 * q) * scale);
+                }
+            }
+        }
+    }
+    for (int64_t c0 = (int64_t)blockIdx.y * 256 + 64 * wave; c0 < W; c0 += (int64_t)gridDim.y * 256) {
+        f32x4 acc[4][4];  // [product][row block]
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t c = c0 + 16 * (x >> 2) + 4 * j + (x & 3);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
+                u32x4 f = {0, 0, 0, 0};
+                if (c < W) {
+                    if constexpr (ROWMAJOR) {
+                        f = load16(factor + c * r, k, r);
+                    } else {
+                        T v[E];
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[e] = k + e < r ? factor[(int64_t)(k + e) * W + c] : (T)0.f;
+                        __builtin_memcpy(&f, v, 16);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < subs) acc[j][i] = mfma16<T>(f, low[b][i], acc[j][i]);
+            }
+        }
+        const int64_t c = c0 + 16 * q;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= subs || 16 * i + x >= t.rows || c >= W) continue;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 old = as_bf16x8(load16(out[i], c + 8 * h, W));
+                    bf16x8 v;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = f32_to_bf16((float)old[e] + acc[2 * h + e / 4][i][e % 4]);
+                    store16(out[i], c + 8 * h, W, as_u32x4(v));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 v = __builtin_bit_cast(f32x4, load16(out[i], c + 4 * j, W)) + acc[j][i];
+                    store16(out[i], c + 4 * j, W, __builtin_bit_cast(u32x4, v));
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// pool_grad: sum over a chunk's rows of low[row][i] * wide[row][c]
+// ---------------------------------------------------------------------------
+// D[rank][column]: the A operand is low (lane: rank), the B operand the wide
+// rows (lane: column), both with the rows as k.  A lane loads 16 bytes of a row:
+// bf16, 8 columns of 8 rows (32 rows per step), whose elements j make product
+// j's operand: columns 8 x + j.  f32: 4 columns of one row, 4 rows a step.
+template <typename T, int RB>
+__device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolParams &p, const Tile &t, int block) {
+    constexpr int E = 16 / sizeof(T), ROWS = sizeof(T) == 2 ? 8 : 1;  // columns and rows of a lane's step
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    const int r = p.r, W = p.wide;
+    const int64_t c = ((int64_t)block * 4 + wave) * 16 * E + E * x;
+    if (c - E * x >= W) return;
+    f32x4 acc[RB][E];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < t.rows; i0 += 4 * ROWS) {
+        u32x4 d[ROWS];
+        float low[RB][ROWS];
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) {
+            const int i = i0 + ROWS * q + e;
+            const int token = token_of(p, t, i);
+            const bool live = i < t.rows;
+            d[e] = live ? load16(static_cast<const T *>(p.x) + token * p.ldx, c, W) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                float v = 0.f;
+                if (live && 16 * b + x < r)
+                    for (int s = 0; s < p.splits; ++s) v += p.low[((int64_t)s * p.T + token) * r + 16 * b + x];
+                low[b][e] = v;
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            u32x4 terms[RB][3];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) split_terms(low[b], terms[b]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                bf16x8 col;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) col[e] = as_bf16x8(d[e])[j];
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) acc[b][j] = mfma_16x16x32(as_bf16x8(terms[b][k]), col, acc[b][j]);
+            }
+        } else {
+            const f32x4 v = __builtin_bit_cast(f32x4, d[0]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) acc[b][j] = mfma_16x16x4_f32(low[b][0], v[j], acc[b][j]);
+        }
+    }
+    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    const int slot = t.slot >= 0 ? v.slot0[t.adapter] + t.slot : -1;
+    if (slot >= g.slots || (t.slot >= 0 && slot < 0)) return;  // not of a plan that this library made
+    float *out = slot >= 0 ? g.part + slot * (int64_t)r * W : g.out + t.adapter * (int64_t)r * W;
+    const float scale = slot >= 0 ? 1.f : p.scale[t.adapter];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int i = 16 * b + 4 * q;
+        if (g.transpose) {  // [wide][r]
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (c + j < W) store_f4(out + (c + j) * r + i, r - i, acc[b][j] * scale);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i + e >= r) continue;
+                float *row = out + (int64_t)(i + e) * W;
+#pragma unroll
+                for (int j = 0; j < E; j += 4)
+                    store_f4(row + c + j, (int)std::min<int64_t>(4, W - c - j),
+                             f32x4{acc[b][j][e], acc[b][j + 1][e], acc[b][j + 2][e], acc[b][j + 3][e]} * scale);
+            }
+        }
+    }
+}
+
+template <typename T, int RB>
+__global__ __launch_bounds__(256) void pool_grad_kernel(PoolParams pa, PoolGradParams ga, PoolParams pb,
+                                                        PoolGradParams gb) {
+    Tile t;
+    if (!tile_of(pa, true, blockIdx.x, t) || t.adapter < 0) return;
+    if ((int)blockIdx.y < ga.blocks)
+        grad_chunk<T, RB>(ga, pa, t, blockIdx.y);
+    else
+        grad_chunk<T, RB>(gb, pb, t, blockIdx.y - ga.blocks);
+}
+
+// Adapters of several chunks: the partial sums in order, times the scale;
+// adapters without tokens: zeros.  grid (adapters, columns of 1024 elements).
+__global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGradParams ga, PoolGradParams gb,
+                                                          int64_t na, int64_t nb) {
+    const int a = blockIdx.x;
+    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    if (v.head[2] != p.T || v.head[3] != p.L) return;
+    const int n = v.count[a], first = v.slot0[a], chunks = (n + kChunk - 1) / kChunk;
+    if (chunks == 1) return;
+    if (chunks > 1 && (first < 0 || first > ga.slots - chunks)) return;
+    const float scale = p.scale[a];
+    for (int64_t e = (int64_t)blockIdx.y * 256 + threadIdx.x; e < na + nb; e += (int64_t)gridDim.y * 256) {
+        const bool is_a = e < na;
+        const int64_t at = is_a ? e : e - na, size = is_a ? na : nb;
+        float s = 0.f;
+        for (int k = 0; k < chunks; ++k) s += (is_a ? ga.part : gb.part)[(first + k) * size + at];
+        (is_a ? ga.out : gb.out)[a * size + at] = chunks ? s * scale : 0.f;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+// Ranges of the wide axis: enough workgroups for two rounds of the chip, none
+// under 256 columns.
+int down_splits(int T, int L, int W) {
+    const int64_t tiles = std::max<int64_t>(1, most_tiles(T, L, kRows));
+    const int64_t want = (2 * (int64_t)device_cu_count() + tiles - 1) / tiles;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), W / 256));
+}
+// Partial gradients: chunks of adapters with more than one, at most two for each full one
+int64_t grad_slots(int T) { return 2 * ((int64_t)T / kChunk); }
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+size_t low_bytes(int T, int r, int splits) { return align256((size_t)splits * T * r * sizeof(float)); }
+
+template <typename T, bool ROWMAJOR>
+hipError_t down_t(const PoolParams &p, hipStream_t s) {
+    const dim3 grid((unsigned)most_tiles(p.T, p.L, kRows), p.splits), block(256);
+    switch ((p.r + 15) / 16) {
+        case 1: hipLaunchKernelGGL((pool_down_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
+        case 2: hipLaunchKernelGGL((pool_down_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
+        case 3: hipLaunchKernelGGL((pool_down_kernel<T, 3, ROWMAJOR>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((pool_down_kernel<T, 4, ROWMAJOR>), grid, block, 0, s, p); break;
+    }
+    return hipGetLastError();
+}
+template <typename T, bool ROWMAJOR>
+hipError_t up_t(const PoolParams &p, hipStream_t s) {
+    const int64_t blocks = ((int64_t)p.wide + 255) / 256;
+    const dim3 grid((unsigned)most_tiles(p.T, p.L, kRows), (unsigned)std::min<int64_t>(blocks, 32768)), block(256);
+    switch ((p.r + 15) / 16) {
+        case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
+        case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
+        case 3: hipLaunchKernelGGL((pool_up_kernel<T, 3, ROWMAJOR>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((pool_up_kernel<T, 4, ROWMAJOR>), grid, block, 0, s, p); break;
+    }
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t grad_t(const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb, const PoolGradParams &gb,
+                  hipStream_t s) {
+    const dim3 grid((unsigned)most_tiles(pa.T, pa.L, kChunk), ga.blocks + gb.blocks), block(256);
+    switch ((pa.r + 15) / 16) {
+        case 1: hipLaunchKernelGGL((pool_grad_kernel<T, 1>), grid, block, 0, s, pa, ga, pb, gb); break;
+        case 2: hipLaunchKernelGGL((pool_grad_kernel<T, 2>), grid, block, 0, s, pa, ga, pb, gb); break;
+        case 3: hipLaunchKernelGGL((pool_grad_kernel<T, 3>), grid, block, 0, s, pa, ga, pb, gb); break;
+        default: hipLaunchKernelGGL((pool_grad_kernel<T, 4>), grid, block, 0, s, pa, ga, pb, gb); break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t prepare_pool_kernels() {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(&pool_plan_kernel),
+                               hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (kPlanWaves * (kPoolMaxAdapters + 1) + 3 * (kPoolMaxAdapters + 2)) * (int)sizeof(int));
+}
+
+size_t pool_plan_bytes(int T, int L) { return (size_t)plan_words(T, L) * sizeof(int); }
+
+hipError_t launch_pool_plan(const int *index, int T, int L, int *plan, hipStream_t s) {
+    const size_t lds = (size_t)(kPlanWaves * (L + 1) + 3 * (L + 2)) * sizeof(int);
+    hipLaunchKernelGGL(pool_plan_kernel, dim3(1), dim3(1024), lds, s, index, T, L, plan);
+    return hipGetLastError();
+}
+
+size_t pool_fwd_workspace_bytes(const PoolCall &c) {
+    const int splits = down_splits(c.T, c.L, c.K);
+    return splits > 1 ? low_bytes(c.T, c.r, splits) : 0;
+}
+
+size_t pool_bwd_workspace_bytes(const PoolCall &c) {
+    return low_bytes(c.T, c.r, down_splits(c.T, c.L, c.M)) +
+           align256((size_t)grad_slots(c.T) * c.r * ((size_t)c.K + c.M) * sizeof(float));
+}
+
+static PoolParams pool_params(const PoolCall &c) {
+    PoolParams p{};
+    p.plan = c.plan;
+    p.scale = c.scale;
+    p.T = c.T;
+    p.L = c.L;
+    p.r = c.r;
+    return p;
+}
+
+hipError_t launch_pool_fwd(const PoolCall &c, int dtype, hipStream_t s) {
+    if (c.T == 0) return hipSuccess;
+    PoolParams p = pool_params(c);
+    p.splits = down_splits(c.T, c.L, c.K);
+    p.x = c.x;
+    p.ldx = c.ldx;
+    p.factor = c.a;
+    p.wide = c.K;
+    p.low = p.splits > 1 ? static_cast<float *>(c.work) : c.u;
+    hipError_t e = dtype == 0 ? down_t<bf16, true>(p, s) : down_t<float, true>(p, s);
+    if (e != hipSuccess) return e;
+    p.factor = c.b;
+    p.wide = c.M;
+    p.y = c.y;
+    p.ldy = c.ldy;
+    p.low_out = p.splits > 1 ? c.u : nullptr;
+    return dtype == 0 ? up_t<bf16, true>(p, s) : up_t<float, true>(p, s);
+}
+
+hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
+    const bool bf = dtype == 0;
+    PoolParams pv = pool_params(c);  // v, from dy
+    pv.splits = down_splits(c.T, c.L, c.M);
+    pv.low = static_cast<float *>(c.work);
+    hipError_t e = hipSuccess;
+    PoolParams pa = pv, pb = pv;  // the gradients' products
+    PoolGradParams ga{}, gb{};
+    float *part = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
+    const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
+    const int cols = bf ? 512 : 256;
+    ga.out = c.da;
+    ga.slots = gb.slots = (int)grad_slots(c.T);
+    ga.part = part;
+    ga.blocks = (c.K + cols - 1) / cols;
+    gb.out = c.db;
+    gb.part = part + ga.slots * na;
+    gb.blocks = (c.M + cols - 1) / cols;
+    gb.transpose = 1;
+    if (c.T > 0) {
+        pv.x = c.dy;
+        pv.ldx = c.lddy;
+        pv.factor = c.b;
+        pv.wide = c.M;
+        if ((e = bf ? down_t<bf16, false>(pv, s) : down_t<float, false>(pv, s)) != hipSuccess) return e;
+        if (c.dx) {
+            PoolParams px = pv;
+            px.factor = c.a;
+            px.wide = c.K;
+            px.y = c.dx;
+            px.ldy = c.lddx;
+            if ((e = bf ? up_t<bf16, false>(px, s) : up_t<float, false>(px, s)) != hipSuccess) return e;
+        }
+        pa.x = c.x;
+        pa.ldx = c.ldx;
+        pa.wide = c.K;
+        pb.x = c.dy;
+        pb.ldx = c.lddy;
+        pb.wide = c.M;
+        pb.low = c.u;
+        pb.splits = 1;
+        if (c.da && (e = bf ? grad_t<bf16>(pa, ga, pb, gb, s) : grad_t<float>(pa, ga, pb, gb, s)) != hipSuccess)
+            return e;
+    }
+    if (!c.da) return hipSuccess;
+    const int64_t per = (na + nb + 1023) / 1024;
+    hipLaunchKernelGGL(pool_reduce_kernel, dim3(c.L, (unsigned)std::min<int64_t>(per, 256)), dim3(256), 0, s, pa, ga,
+                       gb, na, nb);
+    return hipGetLastError();
+}
+
+}  // namespace fa

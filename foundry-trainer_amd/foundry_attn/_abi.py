@@ -37,6 +37,8 @@ EXPORTED = [
     "fa_gated_ln_mod_fwd", "fa_ln_mod_bwd_gate", "fa_gemm_bf16",
     "fa_layer_norm_fwd", "fa_layer_norm_bwd", "fa_layer_norm_bwd_workspace_size",
     "fa_muon_step_many", "fa_muon_step_many_workspace_size",
+    "fa_lora_pool_plan_size", "fa_lora_pool_plan", "fa_lora_pool_fwd_workspace_size", "fa_lora_pool_fwd",
+    "fa_lora_pool_bwd_workspace_size", "fa_lora_pool_bwd",
 ]
 
 
@@ -111,6 +113,22 @@ class LoraBwdArgs(ctypes.Structure):
         ("ldx", ctypes.c_int64), ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
     ]
+
+
+class LoraPoolArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("tokens", ctypes.c_int32), ("in_features", ctypes.c_int32),
+        ("out_features", ctypes.c_int32), ("rank", ctypes.c_int32), ("adapters", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p), ("plan", ctypes.c_void_p), ("plan_bytes", ctypes.c_size_t),
+        ("u", ctypes.c_void_p), ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LoraPoolBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", LoraPoolArgs), ("dy", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("da", ctypes.c_void_p),
+                ("db", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("ldx", ctypes.c_int64)]
 
 
 class LnModArgs(ctypes.Structure):
@@ -301,10 +319,21 @@ def lib() -> ctypes.CDLL:
                      ("fa_swiglu_fwd", SwigluArgs), ("fa_swiglu_bwd", SwigluBwdArgs),
                      ("fa_lora_down", LoraDownArgs), ("fa_lora_up", LoraUpArgs), ("fa_lora_grad", LoraGradArgs),
                      ("fa_gemm_bf16", GemmArgs), ("fa_layer_norm_fwd", LayerNormArgs),
-                     ("fa_layer_norm_bwd", LayerNormBwdArgs)):
+                     ("fa_layer_norm_bwd", LayerNormBwdArgs), ("fa_lora_pool_fwd", LoraPoolArgs),
+                     ("fa_lora_pool_bwd", LoraPoolBwdArgs)):
         fn = getattr(L, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
+    L.fa_lora_pool_plan_size.restype = ctypes.c_size_t
+    L.fa_lora_pool_plan_size.argtypes = [ctypes.c_int32, ctypes.c_int32]
+    L.fa_lora_pool_plan.restype = ctypes.c_int
+    L.fa_lora_pool_plan.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t,
+                                    ctypes.c_void_p]
+    for name, st in (("fa_lora_pool_fwd_workspace_size", LoraPoolArgs),
+                     ("fa_lora_pool_bwd_workspace_size", LoraPoolBwdArgs)):
+        fn = getattr(L, name)
+        fn.restype = ctypes.c_size_t
+        fn.argtypes = [ctypes.POINTER(st)]
     L.fa_layer_norm_bwd_workspace_size.restype = ctypes.c_size_t
     L.fa_layer_norm_bwd_workspace_size.argtypes = [ctypes.POINTER(LayerNormBwdArgs)]
     L.fa_lora_grad_workspace_size.restype = ctypes.c_size_t

@@ -10,6 +10,7 @@ the reference's own code:
   qk_prologue        apply_rope(rms_norm(x, w)) written into the joint buffer
                      (lib.rs:45-58, 122-129, 363-365)
   lora_fwd/lora_bwd  the adapter term of linear_scaled (lib.rs:270-287)
+  lora_pool*         that term for tokens of many adapters at once
 
 Every call goes through libfoundry_attn.so on the tensors' HIP device and the
 current torch stream.  Tensors are [B, S, H, D] (or the reference's per-sample
@@ -87,6 +88,8 @@ _pack_lora_bwd = _abi.packer(_abi.LoraBwdArgs)
 _pack_lora_down = _abi.packer(_abi.LoraDownArgs)
 _pack_lora_up = _abi.packer(_abi.LoraUpArgs)
 _pack_lora_grad = _abi.packer(_abi.LoraGradArgs)
+_pack_pool = _abi.packer(_abi.LoraPoolArgs)
+_pack_pool_bwd = _abi.packer(_abi.LoraPoolBwdArgs)
 
 
 def _keep(key_keep: Optional[torch.Tensor], B: int, S: int, dev) -> Optional[torch.Tensor]:
@@ -614,3 +617,144 @@ def lora_grad_many(items):
     check(_abi.entry("fa_lora_grad_many", ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p)(
         arr, len(built), ws.data_ptr(), ws.numel(), _stream(built[0][1])))
     return [g for _, g in built]
+
+
+# ---------------------------------------------------------------------------
+# a pool of adapters beside one shared projection
+# ---------------------------------------------------------------------------
+class LoraPoolPlan:
+    """Tokens sorted by adapter (lora_pool_plan), on the device."""
+
+    __slots__ = ("tokens", "adapters", "data")
+
+    def __init__(self, tokens: int, adapters: int, data: torch.Tensor):
+        self.tokens, self.adapters, self.data = tokens, adapters, data
+
+    def update(self, index) -> "LoraPoolPlan":
+        """The plan of another index of as many tokens, in the same memory."""
+        if index.shape != (self.tokens,) or index.device != self.data.device:
+            raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"index must be [{self.tokens}] on {self.data.device}")
+        _plan_call(index, self)
+        torch.autograd.graph.increment_version(self.data)
+        return self
+
+
+def _plan_call(index, plan: LoraPoolPlan) -> None:
+    if index.dtype != torch.int32 or not index.is_contiguous():
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "index must be contiguous int32")
+    check(lib().fa_lora_pool_plan(index.data_ptr(), plan.tokens, plan.adapters, plan.data.data_ptr(),
+                                  plan.data.numel(), _stream(index)))
+
+
+def lora_pool_plan(index, adapters: int) -> LoraPoolPlan:
+    """The plan of a batch for lora_pool_fwd and lora_pool_bwd: index [T] int32
+    on the device gives each token's adapter, in any order; tokens with an index
+    outside 0..adapters-1 have none.  One launch, nothing read back; it serves
+    every projection that sees these tokens."""
+    if index.dim() != 1 or not index.is_cuda:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "index must be a 1-D device tensor")
+    tokens, adapters = index.shape[0], int(adapters)
+    if not 1 <= adapters <= 2048 or tokens > 1 << 28:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{adapters} adapters, {tokens} tokens: 1..2048 and up to 2^28")
+    size = lib().fa_lora_pool_plan_size(tokens, adapters)
+    plan = LoraPoolPlan(tokens, adapters, torch.empty(size, dtype=torch.uint8, device=index.device))
+    _plan_call(index, plan)
+    return plan
+
+
+def _pool_rows(t, tokens: int, n: int, like, name: str):
+    if t.shape != (tokens, n) or (n > 1 and t.stride(1) != 1) or t.dtype != like.dtype or t.device != like.device:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
+                               f"{name} must be {like.dtype} [{tokens}, {n}] with contiguous rows on {like.device}")
+    return t
+
+
+def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u) -> tuple:
+    """LoraPoolArgs' values in field order, up to y."""
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or not x.is_cuda:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "x must be [T, K] on the device, a [L, r, K], b [L, M, r]")
+    T, K = x.shape
+    L, r = a.shape[:2]
+    M = b.shape[1]
+    if a.shape != (L, r, K) or b.shape != (L, M, r):
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "a must be [L, r, K], b [L, M, r]")
+    dev, dt = x.device, x.dtype
+    for name, t in (("a", a), ("b", b)):
+        if t.dtype != dt or t.device != dev or not t.is_contiguous():
+            raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{name} must be contiguous {dt} on {dev}")
+    if scales.shape != (L,) or scales.dtype != torch.float32 or not scales.is_contiguous() or scales.device != dev:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"scales must be contiguous float32 [{L}] on {dev}")
+    if plan.tokens != T or plan.adapters != L or plan.data.device != dev:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"the plan is of {plan.tokens} tokens and {plan.adapters} "
+                                                        f"adapters, the call of {T} and {L}")
+    if u.shape != (T, r) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"u must be contiguous float32 [{T}, {r}] on {dev}")
+    _pool_rows(x, T, K, x, "x")
+    return (_dtype_code(x), T, K, M, r, L, x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
+            plan.data.data_ptr(), plan.data.numel(), u.data_ptr())
+
+
+def lora_pool_fwd(x, a, b, y, scales, plan: LoraPoolPlan):
+    """y[t] += scales[i] B_i (A_i x[t]) in place, i the token's adapter; rows of
+    tokens without one stay.  x [T, K], a [L, r, K], b [L, M, r], y [T, M], scales
+    [L] f32; rank 1..64 (pad lower ranks with zeros).  Returns u = A_i x (f32
+    [T, r], zero rows without an adapter) for the backward."""
+    u = torch.empty((x.shape[0], a.shape[1]), dtype=torch.float32, device=x.device)
+    head = _pool_args(x, a, b, scales, plan, u)
+    _pool_rows(y, x.shape[0], b.shape[1], x, "y")
+    head += (y.data_ptr(), y.stride(0))
+    stream = _stream(x)
+    need = _abi.entry("fa_lora_pool_fwd_workspace_size", size=True)(_pack_pool(*head, 0, 0))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _abi.call("fa_lora_pool_fwd", _pack_pool(*head, _ptr(ws), need), stream)
+    return u
+
+
+def lora_pool_bwd(x, a, b, u, dy, scales, plan: LoraPoolPlan, dx=None, want_factors: bool = True):
+    """(da, db) in f32, [L, r, K] and [L, M, r], of lora_pool_fwd for the upstream
+    gradient dy (zero for adapters without tokens; None each without
+    want_factors); dx[t] += scales[i] A_i^T (B_i^T dy[t]) when given."""
+    head = _pool_args(x, a, b, scales, plan, u)
+    _pool_rows(dy, x.shape[0], b.shape[1], x, "dy")
+    if dx is not None:
+        _pool_rows(dx, x.shape[0], x.shape[1], x, "dx")
+    stream = _stream(x)
+    da = db = None
+    if want_factors:
+        da = torch.empty(a.shape, dtype=torch.float32, device=x.device)
+        db = torch.empty(b.shape, dtype=torch.float32, device=x.device)
+    tail = (dy.data_ptr(), dy.stride(0), _ptr(da), _ptr(db), _ptr(dx), 0 if dx is None else dx.stride(0))
+    size = _abi.entry("fa_lora_pool_bwd_workspace_size", size=True)
+    need = max(size(_pack_pool_bwd(*head, 0, 0, 0, 0, *tail)), 256)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _abi.call("fa_lora_pool_bwd", _pack_pool_bwd(*head, 0, 0, ws.data_ptr(), need, *tail), stream)
+    return da, db
+
+
+class _LoraPoolFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, a, b, base, scales, plan):
+        x2 = x.reshape(-1, x.shape[-1])
+        y = base.clone(memory_format=torch.contiguous_format)
+        a, b = a.contiguous(), b.contiguous()
+        u = lora_pool_fwd(x2, a, b, y.view(-1, y.shape[-1]), scales, plan)
+        ctx.save_for_backward(x2, a, b, u, scales, plan.data)
+        ctx.plan = (plan.tokens, plan.adapters)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, a, b, u, scales, data = ctx.saved_tensors
+        dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
+        dx = torch.zeros_like(x2, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None
+        da, db = lora_pool_bwd(x2, a, b, u, dy2, scales, LoraPoolPlan(*ctx.plan, data), dx=dx,
+                               want_factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        cast = lambda g, t: None if g is None else g.to(t.dtype)
+        return (None if dx is None else dx.view(*dy.shape[:-1], -1), cast(da, a), cast(db, b), dy, None, None)
+
+
+def lora_pool(x, a, b, base, scales, plan: LoraPoolPlan):
+    """Differentiable base + adapter term of lora_pool_fwd: x [..., K], base
+    [..., M] the shared projection's output; gradients for x, a, b and base.
+    plan.update between this and its backward is an error torch reports."""
+    return _LoraPoolFn.apply(x, a, b, base, scales, plan)

@@ -422,6 +422,73 @@ size_t fa_lora_grad_many_workspace_size(const fa_lora_grad_args *args, int32_t c
 fa_status fa_lora_grad_many(const fa_lora_grad_args *args, int32_t count, void *workspace,
                             size_t workspace_bytes, void *stream);
 
+/* ---- a pool of adapters beside one shared projection ---------------------- */
+/* The adapter term of linear_scaled (lib.rs:280-285) for tokens of many
+ * requests, or samples of several adapters trained side by side, at once:
+ * token t belongs to adapter i = index[t], or to none where index[t] is
+ * outside 0..adapters-1.  The reference has one adapter per linear and applies
+ * it to every token; it has no counterpart of these calls.
+ *
+ * fa_lora_pool_plan sorts the tokens by adapter into `plan` (device memory of
+ * fa_lora_pool_plan_size bytes, 16-byte aligned).  It is one launch, reads
+ * nothing back, and serves every projection of the same tokens: a model makes
+ * it once per batch.  It is captured into a graph like any other call, and a
+ * replay sorts what `index` holds then. */
+#define FA_LORA_POOL_MAX_ADAPTERS 2048
+size_t fa_lora_pool_plan_size(int32_t tokens, int32_t adapters);
+fa_status fa_lora_pool_plan(const int32_t *index, int32_t tokens, int32_t adapters, void *plan, size_t plan_bytes,
+                            void *stream);
+
+typedef struct fa_lora_pool_args {
+    int32_t dtype;        /* fa_dtype of x, a, b, y (and dy, dx)               */
+    int32_t tokens;       /* T: 0..2^28, as the plan's                         */
+    int32_t in_features;  /* K: 1..2^22                                        */
+    int32_t out_features; /* M: 1..2^22                                        */
+    int32_t rank;         /* r: 1..64; adapters of lower rank are padded with
+                             zero rows of a and zero columns of b              */
+    int32_t adapters;     /* L: 1..FA_LORA_POOL_MAX_ADAPTERS, as the plan's    */
+    const void *x;        /* [T, K] rows of stride ldx >= K                    */
+    int64_t ldx;
+    const void *a;        /* [L, r, K] contiguous (each a lora_a)              */
+    const void *b;        /* [L, M, r] contiguous (each a lora_b)              */
+    const float *scale;   /* [L] f32 on the device                             */
+    const void *plan;     /* of fa_lora_pool_plan for these tokens             */
+    size_t plan_bytes;
+    float *u;             /* [T, r] f32: A_i x (written by fwd, 0 for tokens
+                             without an adapter; read by bwd)                  */
+    void *y;              /* [T, M] rows of stride ldy >= M (fwd: in/out)      */
+    int64_t ldy;
+    void *workspace;      /* device scratch, 256-byte aligned; may be NULL
+                             where none is asked for                           */
+    size_t workspace_bytes;
+} fa_lora_pool_args;
+
+/* y[t] += scale_i B_i (A_i x[t]); rows of tokens without an adapter stay as
+ * they are.  Any sizes and strides: rows and factors need their element's
+ * alignment only.  Deterministic.  A plan of other tokens or adapters, or
+ * memory that is no plan, gives wrong results but leads to no access outside
+ * the call's tensors. */
+size_t fa_lora_pool_fwd_workspace_size(const fa_lora_pool_args *args);
+fa_status fa_lora_pool_fwd(const fa_lora_pool_args *args, void *stream);
+
+typedef struct fa_lora_pool_bwd_args {
+    fa_lora_pool_args fwd; /* the forward's arguments (y unused), with a
+                             workspace of fa_lora_pool_bwd_workspace_size bytes */
+    const void *dy;       /* [T, M] rows of stride ldy >= M                    */
+    int64_t ldy;
+    float *da;            /* [L, r, K] f32 output, or NULL together with db    */
+    float *db;            /* [L, M, r] f32 output                              */
+    void *dx;             /* NULL, or [T, K] rows of stride ldx >= K:
+                             dx[t] += scale_i A_i^T (B_i^T dy[t])              */
+    int64_t ldx;
+} fa_lora_pool_bwd_args;
+
+/* da_i = scale_i sum_t (B_i^T dy[t]) x[t]^T and db_i = scale_i sum_t dy[t]
+ * u[t]^T over the tokens of adapter i (zero for adapters without any), and the
+ * adapters' share of the input's gradient.  Deterministic. */
+size_t fa_lora_pool_bwd_workspace_size(const fa_lora_pool_bwd_args *args);
+fa_status fa_lora_pool_bwd(const fa_lora_pool_bwd_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
