@@ -12,7 +12,7 @@
 //   pool_down   64 rows x a range of the wide axis: u or v, f32, over `splits`
 //               ranges that the reader adds in order
 //   pool_up     64 rows x 256 columns: y or dx
-//   pool_grad   a chunk x 512 (f32: 256) columns of dA or dB: straight to the
+//   pool_grad   a chunk x 256 (f32: 128) columns of dA or dB: straight to the
 //               result where the adapter has one chunk, else a partial sum
 //   pool_reduce the partial sums in order, and zeros for adapters without tokens
 // u and v are f32 between the kernels.  bf16 products (v_mfma_f32_16x16x32) take
@@ -24,6 +24,7 @@
 
 #include "fa_device.hpp"
 #include "fa_kernels.hpp"
+#include "fa_lds.hpp"
 
 namespace fa {
 namespace {
@@ -32,71 +33,80 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 constexpr int kRows = 64;     // of a row tile
-constexpr int kChunk = 256;   // rows of a gradient chunk
+constexpr int kChunk = 256;   // rows of a gradient chunk: whole tiles
 constexpr int kPlanWaves = 16;
 
 // ---------------------------------------------------------------------------
 // the plan: int32 words
 // ---------------------------------------------------------------------------
 struct Tile {
-    int start, rows, adapter, slot;  // rows perm[start .. start + rows); adapter -1: none
+    int tile, rows, adapter, slot;  // rows token[64 * tile .. + rows); adapter -1: none
 };
 struct PlanView {
-    int *head;    // tiles, chunks
-    int *perm;    // [T] tokens sorted by adapter, those without one last
+    int *head;    // tiles, chunks, T, L
     int *count;   // [L] tokens of each adapter
     int *slot0;   // [L] its first partial gradient; -1: none (at most one chunk)
     Tile *tiles, *chunks;
+    int *token;   // sorted by adapter, those without one last; each adapter begins a tile
 };
 __host__ __device__ inline int64_t most_tiles(int64_t T, int64_t L, int rows) {
     return (T + rows - 1) / rows + (L + 1 < T ? L + 1 : T);
 }
 __host__ __device__ inline int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
 __host__ __device__ inline int64_t plan_words(int64_t T, int64_t L) {
-    return 4 + round4(T) + 2 * round4(L) + 4 * (most_tiles(T, L, kRows) + most_tiles(T, L, kChunk));
+    return 4 + 2 * round4(L) + (4 + kRows) * most_tiles(T, L, kRows) + 4 * most_tiles(T, L, kChunk);
 }
 __host__ __device__ inline PlanView plan_view(int *p, int64_t T, int64_t L) {
     PlanView v;
     v.head = p;
-    v.perm = p + 4;
-    v.count = v.perm + round4(T);
+    v.count = p + 4;
     v.slot0 = v.count + round4(L);
     v.tiles = reinterpret_cast<Tile *>(v.slot0 + round4(L));
     v.chunks = v.tiles + most_tiles(T, L, kRows);
+    v.token = reinterpret_cast<int *>(v.chunks + most_tiles(T, L, kChunk));
     return v;
 }
 
 // One workgroup.  Wave w holds the w-th sixteenth of the tokens; hist[w][a]
-// first counts its tokens of adapter a (a = L: none), then holds where in perm
-// they begin.
-__global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T, int L, int *plan) {
+// first counts its tokens of adapter a (a = L: none), then holds where in
+// `token` they begin.  The lanes of a wave that hold the same adapter find each
+// other by one ballot per bit of its number: 64 tokens of 48 adapters took 5 us
+// by one ballot per adapter, and the whole plan 11.5 us.
+__global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T, int L, int bits, int *plan) {
     extern __shared__ int hist[];  // [kPlanWaves][L + 1], then [3][L + 2]: rows, tiles and chunks before adapter a
     __shared__ int carry[kPlanWaves][4], total[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, A = L + 1;
     int *rows0 = hist + kPlanWaves * A, *tiles0 = rows0 + L + 2, *chunks0 = tiles0 + L + 2;
     const PlanView v = plan_view(plan, T, L);
-    for (int i = tid; i < kPlanWaves * A; i += 1024) hist[i] = 0;
-    __syncthreads();
+    constexpr int kKept = 8;  // of a lane's adapters stay in registers
     const int64_t share = (((int64_t)T + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
     const int64_t t0 = wave * share, t1 = std::min<int64_t>(T, t0 + share);
     auto adapter_of = [&](int64_t t) {
-        const int a = t < t1 ? index[t] : -2;
+        const int a = t < t1 ? index[t] : 0;
         return t >= t1 ? -1 : (a < 0 || a >= L ? L : a);
     };
-    // f(adapter, its lanes) for each adapter among the wave's next 64 tokens
-    auto each = [&](int a, auto f) {
-        uint64_t left = __ballot(a >= 0);
-        while (left) {
-            const int cur = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
-            const uint64_t same = __ballot(a == cur);
-            f(cur, same);
-            left &= ~same;
+    int kept[kKept];
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) kept[k] = adapter_of(t0 + 64 * k + lane);
+    for (int i = tid; i < kPlanWaves * A; i += 1024) hist[i] = 0;
+    __syncthreads();
+    // lanes that hold the same adapter as this one
+    auto peers = [&](int a) {
+        uint64_t same = __ballot(a >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot(a >> b & 1);
+            same &= a >> b & 1 ? set : ~set;
         }
+        return same;
     };
-    for (int64_t t = t0; t < t1; t += 64)
-        each(adapter_of(t + lane), [&](int a, uint64_t same) {
-            hist[wave * A + a] += __popcll(same);  // every lane the same
-        });
+    auto first_pass = [&](int a) {
+        const uint64_t same = peers(a);
+        if (a >= 0 && lane == __builtin_ctzll(same)) hist[wave * A + a] += __popcll(same);
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+        if (t0 + 64 * k < t1) first_pass(kept[k]);
+    for (int64_t t = t0 + 64 * kKept; t < t1; t += 64) first_pass(adapter_of(t + lane));
     __syncthreads();
     // exclusive sums over adapters of rows, tiles, chunks and partial slots:
     // thread i holds the E adapters from i * E on
@@ -134,40 +144,52 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
         tiles0[a] = before[1];
         chunks0[a] = before[2];
         const int slot0 = before[3];
-        const int n = add(a, before);
-        if (a < L) {
-            v.count[a] = n;
-            v.slot0[a] = before[3] > slot0 ? slot0 : -1;
-        }
-        if (a == L) {
-            rows0[A] = before[0];
-            tiles0[A] = before[1];
-            chunks0[A] = before[2];
-            for (int k = 0; k < 4; ++k) total[k] = before[k];
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        v.head[0] = total[1];
-        v.head[1] = total[2];
-        v.head[2] = T;
-        v.head[3] = L;
-    }
-    for (int a = tid; a < A; a += 1024) {
-        int at = rows0[a];
+        int at = before[1] * kRows;
         for (int w = 0; w < kPlanWaves; ++w) {
             const int n = hist[w * A + a];
             hist[w * A + a] = at;
             at += n;
         }
+        const int n = at - before[1] * kRows, c = a < L ? (n + kChunk - 1) / kChunk : 0;
+        before[0] += n;
+        before[1] += (n + kRows - 1) / kRows;
+        before[2] += c;
+        before[3] += c > 1 ? c : 0;
+        if (a < L) {
+            v.count[a] = n;
+            v.slot0[a] = c > 1 ? slot0 : -1;
+        } else {
+            rows0[A] = before[0];
+            tiles0[A] = before[1];
+            chunks0[A] = before[2];
+            total[0] = before[1];
+            total[1] = before[2];
+        }
     }
     __syncthreads();
-    for (int64_t t = t0; t < t1; t += 64)
-        each(adapter_of(t + lane), [&](int a, uint64_t same) {
-            const int at = hist[wave * A + a];
-            if (same >> lane & 1) v.perm[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)(t + lane);
-            hist[wave * A + a] = at + __popcll(same);
-        });
+    if (tid == 0) {
+        v.head[0] = total[0];
+        v.head[1] = total[1];
+        v.head[2] = T;
+        v.head[3] = L;
+    }
+    auto second_pass = [&](int a, int64_t t) {
+        const uint64_t same = peers(a);
+        if (a < 0) return;
+        const int at = hist[wave * A + a];
+        v.token[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)t;
+        if (lane == __builtin_ctzll(same)) hist[wave * A + a] = at + __popcll(same);
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+        if (t0 + 64 * k < t1) {
+            second_pass(kept[k], t0 + 64 * k + lane);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    for (int64_t t = t0 + 64 * kKept; t < t1; t += 64) {
+        second_pass(adapter_of(t + lane), t + lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     auto find = [&](const int *first, int i) {  // the adapter a with first[a] <= i < first[a + 1]
         int lo = 0, hi = A - 1;
         while (lo < hi) {
@@ -177,32 +199,45 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
         }
         return lo;
     };
-    for (int i = tid; i < total[1]; i += 1024) {
-        const int a = find(tiles0, i), k = i - tiles0[a], start = rows0[a] + k * kRows;
-        v.tiles[i] = Tile{start, std::min(kRows, rows0[a + 1] - start), a < L ? a : -1, 0};
+    for (int i = tid; i < total[0]; i += 1024) {
+        const int a = find(tiles0, i), k = i - tiles0[a];
+        v.tiles[i] = Tile{i, std::min(kRows, rows0[a + 1] - rows0[a] - k * kRows), a < L ? a : -1, 0};
     }
-    for (int i = tid; i < total[2]; i += 1024) {
-        const int a = find(chunks0, i), k = i - chunks0[a], start = rows0[a] + k * kChunk;
-        v.chunks[i] = Tile{start, std::min(kChunk, rows0[a + 1] - start), a, chunks0[a + 1] - chunks0[a] > 1 ? k : -1};
+    for (int i = tid; i < total[1]; i += 1024) {
+        const int a = find(chunks0, i), k = i - chunks0[a];
+        v.chunks[i] = Tile{tiles0[a] + k * (kChunk / kRows), std::min(kChunk, rows0[a + 1] - rows0[a] - k * kChunk), a,
+                           chunks0[a + 1] - chunks0[a] > 1 ? k : -1};
     }
 }
 
-// A tile of the plan as the kernels trust it: nothing of it leads outside the
-// call's tensors, whatever memory the plan was given.
-__device__ __forceinline__ bool tile_of(const PoolParams &p, bool chunk, int i, Tile &t) {
-    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
-    if (v.head[2] != p.T || v.head[3] != p.L) return false;
-    const int n = chunk ? v.head[1] : v.head[0];
-    if (i >= n) return false;
-    t = (chunk ? v.chunks : v.tiles)[i];
-    const int most = chunk ? kChunk : kRows;
-    return t.start >= 0 && t.rows > 0 && t.rows <= most && t.start <= p.T - t.rows && t.adapter < p.L;
+// Tile or chunk i of the plan as the kernels trust it: nothing of it leads
+// outside the call's tensors, whatever memory the plan was given.
+__device__ __forceinline__ bool tile_of(const PoolParams &p, const PlanView &v, bool chunk, int i, Tile &t) {
+    // all loads at once: the tile's place holds some word, whether or not there is such a tile
+    const u32x4 head = *reinterpret_cast<const u32x4 *>(v.head);
+    const u32x4 w = *reinterpret_cast<const u32x4 *>((chunk ? v.chunks : v.tiles) + i);
+    t = __builtin_bit_cast(Tile, w);
+    const int n = (int)(chunk ? head[1] : head[0]), most = chunk ? kChunk : kRows;
+    return (int)head[2] == p.T && (int)head[3] == p.L && i < n && t.tile >= 0 && t.rows > 0 && t.rows <= most &&
+           t.tile + (t.rows + kRows - 1) / kRows <= most_tiles(p.T, p.L, kRows) && t.adapter < p.L;
 }
-// Token of row i of a tile; past its end the last one's (read, never written).
-__device__ __forceinline__ int token_of(const PoolParams &p, const Tile &t, int i) {
-    const int *perm = p.plan + 4;
-    const int row = perm[t.start + std::min(i, t.rows - 1)];
+// The token in entry `at` of the plan's list; 0 where it holds no token.
+__device__ __forceinline__ int token_at(const PoolParams &p, const PlanView &v, int64_t at) {
+    const int row = v.token[at];
     return (unsigned)row < (unsigned)p.T ? row : 0;
+}
+// Its tokens, for a lane that reads row 16 i + x of a row tile in its i-th load:
+// rows past the end read the block's first (and are not written).
+__device__ __forceinline__ void tile_tokens(const PoolParams &p, const PlanView &v, int tile, int x, int (&token)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) token[i] = token_at(p, v, (int64_t)tile * kRows + 16 * i + x);
+}
+__device__ __forceinline__ void clamp_tokens(const Tile &t, int x, int (&token)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int first = __builtin_amdgcn_readfirstlane(token[i]);
+        if (16 * i + x >= t.rows) token[i] = first;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -293,13 +328,17 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), STEP = 8 * E;
     __shared__ f32x4 sum[4][RB][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    int token[4];
+    tile_tokens(p, v, blockIdx.x, x, token);
     Tile t;
-    if (!tile_of(p, false, blockIdx.x, t)) return;
+    if (!tile_of(p, v, false, blockIdx.x, t)) return;
+    clamp_tokens(t, x, token);
     const int r = p.r, W = p.wide;
     const int64_t part = (int64_t)blockIdx.y * p.T;
     if (t.adapter < 0) {
         for (int i = threadIdx.x; i < t.rows * r; i += 256)
-            p.low[(part + token_of(p, t, i / r)) * r + i % r] = 0.f;
+            p.low[(part + token_at(p, v, (int64_t)t.tile * kRows + i / r)) * r + i % r] = 0.f;
         return;
     }
     const int subs = (t.rows + 15) / 16;
@@ -307,7 +346,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     const int64_t s0 = steps * blockIdx.y / gridDim.y, s1 = steps * (blockIdx.y + 1) / gridDim.y;
     const T *rows[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = static_cast<const T *>(p.x) + token_of(p, t, 16 * i + x) * p.ldx;
+    for (int i = 0; i < 4; ++i) rows[i] = static_cast<const T *>(p.x) + token[i] * p.ldx;
     const T *factor = static_cast<const T *>(p.factor) + (int64_t)t.adapter * r * W;
     f32x4 acc[RB][4];
 #pragma unroll
@@ -331,13 +370,13 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
                 if constexpr (ROWMAJOR) {
                     f[b][h] = i < r ? load16(factor + (int64_t)i * W, c + E * h, W) : u32x4{0, 0, 0, 0};
                 } else {
-                    T v[E];
+                    T w[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const int64_t m = c + E * h + e;
-                        v[e] = i < r && m < W ? factor[m * r + i] : (T)0.f;
+                        w[e] = i < r && m < W ? factor[m * r + i] : (T)0.f;
                     }
-                    __builtin_memcpy(&f[b][h], v, 16);
+                    __builtin_memcpy(&f[b][h], w, 16);
                 }
             }
         }
@@ -357,123 +396,202 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     __syncthreads();
     // wave i stores rows 16 i .. + 16: ranks 16 b + 4 q .. + 4 of token x
     if (16 * wave + x >= t.rows) return;
-    float *out = p.low + (part + token_of(p, t, 16 * wave + x)) * r;
+    const int mine = wave == 0 ? token[0] : wave == 1 ? token[1] : wave == 2 ? token[2] : token[3];
+    float *out = p.low + (part + mine) * r;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-        f32x4 v = sum[0][b][wave][lane];
+        f32x4 o = sum[0][b][wave][lane];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += sum[w][b][wave][lane];
-        store_f4(out + 16 * b + 4 * q, r - 16 * b - 4 * q, v);
+        for (int w = 1; w < 4; ++w) o += sum[w][b][wave][lane];
+        store_f4(out + 16 * b + 4 * q, r - 16 * b - 4 * q, o);
     }
-}
-
-// Ranks i .. i + 4 of a token's u or v: its `splits` parts in order.
-__device__ __forceinline__ f32x4 low_f4(const PoolParams &p, int token, int i) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s)
-        v += load_f4(p.low + ((int64_t)s * p.T + token) * p.r + i, p.r - i);
-    return v;
 }
 
 // ---------------------------------------------------------------------------
 // pool_up: y += s B u (ROWMAJOR: the factor's rows run along the rank) or
 // dx += s A^T v (A [r][wide])
 // ---------------------------------------------------------------------------
-// D[column][token]: a wave's step is 64 columns in four products; row 4 q + v of
-// product j is column 16 q + 4 j + v, so that a lane ends with 16 consecutive
-// columns of its token.
+// D[column][token]: a wave's step is 64 columns in four products; row 4 q + e of
+// product j is column 16 q + 4 j + e, so that a lane ends with 16 consecutive
+// columns of its token.  The rows of y and the factor of the wave's next step are
+// loaded before this step's products.
+constexpr int kUpStep = 64;                   // columns of a wave's step
+constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
+constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
+
 template <typename T, int RB, bool ROWMAJOR>
 __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
-    constexpr int E = 16 / sizeof(T);
+    constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
+    constexpr int PITCH = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
+    __shared__ float lowsum[kRows][RB * 16 + 4];
+    __shared__ __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    int token[4];
+    tile_tokens(p, v, blockIdx.x, x, token);
+    // four threads a row: its ranks 4 h .. of every 16, the parts in order
+    const int h = threadIdx.x & 3, lrow = threadIdx.x >> 2;
+    const int ltoken = token_at(p, v, (int64_t)blockIdx.x * kRows + lrow);
     Tile t;
-    if (!tile_of(p, false, blockIdx.x, t)) return;
-    const int r = p.r, W = p.wide;
-    const int subs = (t.rows + 15) / 16;
-    if (p.low_out && blockIdx.y == 0) {  // the parts' sum, for the backward
-        for (int i = threadIdx.x; i < t.rows * ((r + 3) / 4); i += 256) {
-            const int token = token_of(p, t, i / ((r + 3) / 4)), k = i % ((r + 3) / 4) * 4;
-            store_f4(p.low_out + (int64_t)token * r + k, r - k, low_f4(p, token, k));
+    if (!tile_of(p, v, false, blockIdx.x, t)) return;
+    clamp_tokens(t, x, token);
+    const int r = p.r, W = p.wide, subs = (t.rows + 15) / 16;
+    const bool live = t.adapter >= 0;
+    if (!live && !(p.low_out && blockIdx.y == 0)) return;
+    const float scale = live ? p.scale[t.adapter] : 0.f;
+    const T *factor = static_cast<const T *>(p.factor) + (int64_t)(live ? t.adapter : 0) * r * W;
+    T *out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = static_cast<T *>(p.y) + token[i] * p.ldy;
+    const int64_t step = (int64_t)gridDim.y * 4 * kUpStep;
+    int64_t c0 = ((int64_t)blockIdx.y * 4 + wave) * kUpStep;
+
+    u32x4 y[4][NY];
+    u32x4 f[ROWMAJOR ? 4 : 1][RB];  // ROWMAJOR: the four products' operands
+    u32x4 g[ROWMAJOR ? 1 : RB][ROWMAJOR ? 1 : 8 / E * 2];  // else rows as they lie, to be staged
+    auto load_y = [&](int64_t at) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < subs) {
+#pragma unroll
+                for (int n = 0; n < NY; ++n) y[i][n] = load16(out[i], at + 16 * q + E * n, W);
+            }
+    };
+    auto load_factor = [&](int64_t at) {
+        if constexpr (ROWMAJOR) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t c = at + 16 * (x >> 2) + 4 * j + (x & 3);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
+                    f[j][b] = c < W ? load16(factor + c * r, k, r) : u32x4{0, 0, 0, 0};
+                }
+            }
+        } else {
+            constexpr int LANES = kUpStep / E;  // lanes of a row
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int n = 0; n < 16 * LANES / 64; ++n) {
+                    const int i = 16 * b + n * (64 / LANES) + lane / LANES;
+                    g[b][n] = i < r ? load16(factor + (int64_t)i * W, at + E * (lane % LANES), W) : u32x4{0, 0, 0, 0};
+                }
+        }
+    };
+    if (live && c0 < W) {
+        load_y(c0);
+        load_factor(c0);
+    }
+    {
+        f32x4 s[RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (lrow < t.rows)
+            for (int k = 0; k < p.splits; ++k)
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                    s[b] += load_f4(p.low + ((int64_t)k * p.T + ltoken) * r + 16 * b + 4 * h, r - 16 * b - 4 * h);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            if (p.low_out && blockIdx.y == 0 && lrow < t.rows)  // the parts' sum, for the backward
+                store_f4(p.low_out + (int64_t)ltoken * r + 16 * b + 4 * h, r - 16 * b - 4 * h, s[b]);
+            *reinterpret_cast<f32x4 *>(&lowsum[lrow][16 * b + 4 * h]) = s[b] * scale;
         }
     }
-    if (t.adapter < 0) return;
-    const float scale = p.scale[t.adapter];
-    const T *factor = static_cast<const T *>(p.factor) + (int64_t)t.adapter * r * W;
+    if (!live) return;
+    __syncthreads();
     // the tokens' operand: bf16 takes the high parts of 16 ranks in lane groups
     // 0 and 1, what they leave in 2 and 3; f32 ranks 4 q .. + 4
     u32x4 low[RB][4];
-    T *out[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int token = token_of(p, t, 16 * i + x);
-        out[i] = static_cast<T *>(p.y) + token * p.ldy;
-        if (i < subs) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                if constexpr (sizeof(T) == 2) {
-                    const int k = 16 * b + 8 * (q & 1);
-                    const f32x4 a = low_f4(p, token, k), c = low_f4(p, token, k + 4);
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        v[j] = a[j] * scale;
-                        v[4 + j] = c[j] * scale;
-                    }
-                    u32x4 terms[2];
-                    split_terms(v, terms);
-                    low[b][i] = q < 2 ? terms[0] : terms[1];
-                } else {
-                    low[b][i] = __builtin_bit_cast(u32x4, low_f4(p, token, 16 * b + 4 * q) * scale);
-                }
+        for (int b = 0; b < RB; ++b) {
+            const float *src = &lowsum[16 * i + x][16 * b];
+            if constexpr (sizeof(T) == 2) {
+                const f32x4 lo = *reinterpret_cast<const f32x4 *>(src + 8 * (q & 1));
+                const f32x4 hi = *reinterpret_cast<const f32x4 *>(src + 8 * (q & 1) + 4);
+                const float w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                u32x4 terms[2];
+                split_terms(w, terms);
+                low[b][i] = q < 2 ? terms[0] : terms[1];
+            } else {
+                low[b][i] = *reinterpret_cast<const u32x4 *>(src + 4 * q);
             }
         }
-    }
-    for (int64_t c0 = (int64_t)blockIdx.y * 256 + 64 * wave; c0 < W; c0 += (int64_t)gridDim.y * 256) {
-        f32x4 acc[4][4];  // [product][row block]
+    char *mine = stage + (ROWMAJOR ? 0 : wave * RB * 16 * PITCH);
+    while (c0 < W) {
+        u32x4 fc[4][RB], yc[4][NY];
+        if constexpr (ROWMAJOR) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int b = 0; b < RB; ++b) fc[j][b] = f[j][b];
+        } else {
+            // through LDS of the wave's own: row i of the factor's 64 columns
+            constexpr int LANES = kUpStep / E;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t c = c0 + 16 * (x >> 2) + 4 * j + (x & 3);
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
-                u32x4 f = {0, 0, 0, 0};
-                if (c < W) {
-                    if constexpr (ROWMAJOR) {
-                        f = load16(factor + c * r, k, r);
+                for (int n = 0; n < 16 * LANES / 64; ++n) {
+                    char *d = mine + (16 * b + n * (64 / LANES) + lane / LANES) * PITCH + 16 * (lane % LANES);
+                    *reinterpret_cast<u32x2 *>(d) = u32x2{g[b][n][0], g[b][n][1]};
+                    *reinterpret_cast<u32x2 *>(d + 8) = u32x2{g[b][n][2], g[b][n][3]};
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    if constexpr (sizeof(T) == 2) {
+                        // lane 4 e + k of 16 points at row e, column 16 k + 4 j; lane m receives column
+                        // 16 (m / 4) + 4 j + m % 4 of the four rows
+                        const uint32_t at = (16 * b + 8 * (q & 1) + (x >> 2)) * PITCH + (16 * (x & 3) + 4 * j) * 2;
+                        fc[j][b] = as_u32x4(lds_read_col_frag(mine, at, at + 4 * PITCH));
                     } else {
-                        T v[E];
+                        const float *src = reinterpret_cast<const float *>(mine);
+                        f32x4 w;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = k + e < r ? factor[(int64_t)(k + e) * W + c] : (T)0.f;
-                        __builtin_memcpy(&f, v, 16);
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = src[(16 * b + 4 * q + e) * (PITCH / 4) + 16 * (x >> 2) + 4 * j + (x & 3)];
+                        fc[j][b] = __builtin_bit_cast(u32x4, w);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < subs) acc[j][i] = mfma16<T>(f, low[b][i], acc[j][i]);
-            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
         const int64_t c = c0 + 16 * q;
+        c0 += step;
+        if (c0 < W) {
+            load_y(c0);
+            load_factor(c0);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (i >= subs || 16 * i + x >= t.rows || c >= W) continue;
-            if constexpr (sizeof(T) == 2) {
+            if (i >= subs) continue;
+            f32x4 acc[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bf16x8 old = as_bf16x8(load16(out[i], c + 8 * h, W));
-                    bf16x8 v;
+            for (int j = 0; j < 4; ++j) {
+                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = f32_to_bf16((float)old[e] + acc[2 * h + e / 4][i][e % 4]);
-                    store16(out[i], c + 8 * h, W, as_u32x4(v));
-                }
-            } else {
+                for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b][i], acc[j]);
+            }
+            if (16 * i + x >= t.rows || c >= W) continue;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 v = __builtin_bit_cast(f32x4, load16(out[i], c + 4 * j, W)) + acc[j][i];
-                    store16(out[i], c + 4 * j, W, __builtin_bit_cast(u32x4, v));
+            for (int n = 0; n < NY; ++n) {
+                if constexpr (sizeof(T) == 2) {
+                    const bf16x8 old = as_bf16x8(yc[i][n]);
+                    bf16x8 o;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = f32_to_bf16((float)old[e] + acc[2 * n + e / 4][e % 4]);
+                    store16(out[i], c + 8 * n, W, as_u32x4(o));
+                } else {
+                    store16(out[i], c + 4 * n, W,
+                            __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, yc[i][n]) + acc[n]));
                 }
             }
         }
@@ -487,58 +605,136 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 // rows (lane: column), both with the rows as k.  A lane loads 16 bytes of a row:
 // bf16, 8 columns of 8 rows (32 rows per step), whose elements j make product
 // j's operand: columns 8 x + j.  f32: 4 columns of one row, 4 rows a step.
+//
+// The chunk's tokens and its low, as the bf16 products take it (three terms,
+// [rank block][term][32-row step][lane group][rank][8 rows]) or in f32 ([row][rank
+// + 1 pad]), lie in LDS for all waves.  Two pairs of waves take every other step
+// each; the second's sums are added through LDS.
+constexpr int kGradRows = 32;  // of a step
+
 template <typename T, int RB>
-__device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolParams &p, const Tile &t, int block) {
-    constexpr int E = 16 / sizeof(T), ROWS = sizeof(T) == 2 ? 8 : 1;  // columns and rows of a lane's step
+struct GradLds {
+    int token[kChunk];
+    union {
+        u32x4 terms[sizeof(T) == 2 ? RB * 3 * kChunk * 2 : 1];  // 16 ranks x kChunk rows = 2 kChunk vectors of 8
+        float low[sizeof(T) == 2 ? 1 : kChunk][RB * 16 + 1];
+        f32x4 sum[2][RB][16 / sizeof(T)][64];
+    };
+};
+
+template <typename T, int RB>
+__device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolParams &p, const PlanView &v,
+                                           const Tile &t, int block, GradLds<T, RB> &lds) {
+    constexpr int E = 16 / sizeof(T), ROWS = 8;  // columns and rows of a lane's step
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
+    const int pair = wave >> 1;
     const int r = p.r, W = p.wide;
-    const int64_t c = ((int64_t)block * 4 + wave) * 16 * E + E * x;
-    if (c - E * x >= W) return;
+    const int64_t base = ((int64_t)block * 2 + (wave & 1)) * 16 * E, c = base + E * x;
+    const int steps = (t.rows + kGradRows - 1) / kGradRows;
+    {
+        const int i = threadIdx.x;
+        const int token = i < t.rows ? token_at(p, v, (int64_t)t.tile * kRows + i) : -1;
+        lds.token[i] = token;
+    }
+    __syncthreads();
+    u32x4 d[ROWS];
+    // bf16: rows 8 q + e of the step; f32: rows 4 e + q
+    auto load_wide = [&](int s) {
+#pragma unroll
+        for (int e = 0; e < ROWS; ++e) {
+            const int token = lds.token[s * kGradRows + (sizeof(T) == 2 ? 8 * q + e : 4 * e + q)];
+            d[e] = token >= 0 ? load16(static_cast<const T *>(p.x) + token * p.ldx, c, W) : u32x4{0, 0, 0, 0};
+        }
+    };
+    const bool any = base < W;
+    if (any && pair < steps) load_wide(pair);
+    if constexpr (sizeof(T) == 2) {
+        // thread: rank i % 16, rows 8 (i / 16) .. + 8
+        for (int i = threadIdx.x; i < 2 * kChunk && i / 16 * 8 < steps * kGradRows; i += 256) {
+            const int rank = i % 16, row = i / 16 * 8;
+            float low[RB][8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int token = lds.token[row + e];
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    float w = 0.f;
+                    if (token >= 0 && 16 * b + rank < r)
+                        for (int k = 0; k < p.splits; ++k) w += p.low[((int64_t)k * p.T + token) * r + 16 * b + rank];
+                    low[b][e] = w;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                u32x4 terms[3];
+                split_terms(low[b], terms);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) lds.terms[(b * 3 + k) * 2 * kChunk + i] = terms[k];
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < kChunk * RB * 16; i += 256) {
+            const int row = i / (RB * 16), rank = i % (RB * 16), token = lds.token[row];
+            float w = 0.f;
+            if (token >= 0 && rank < r)
+                for (int k = 0; k < p.splits; ++k) w += p.low[((int64_t)k * p.T + token) * r + rank];
+            lds.low[row][rank] = w;
+        }
+    }
+    __syncthreads();
     f32x4 acc[RB][E];
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int j = 0; j < E; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < t.rows; i0 += 4 * ROWS) {
-        u32x4 d[ROWS];
-        float low[RB][ROWS];
+    if (any)
+        for (int s = pair; s < steps; s += 2) {
+            u32x4 w[ROWS];
 #pragma unroll
-        for (int e = 0; e < ROWS; ++e) {
-            const int i = i0 + ROWS * q + e;
-            const int token = token_of(p, t, i);
-            const bool live = i < t.rows;
-            d[e] = live ? load16(static_cast<const T *>(p.x) + token * p.ldx, c, W) : u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                float v = 0.f;
-                if (live && 16 * b + x < r)
-                    for (int s = 0; s < p.splits; ++s) v += p.low[((int64_t)s * p.T + token) * r + 16 * b + x];
-                low[b][e] = v;
-            }
-        }
-        if constexpr (sizeof(T) == 2) {
-            u32x4 terms[RB][3];
-#pragma unroll
-            for (int b = 0; b < RB; ++b) split_terms(low[b], terms[b]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                bf16x8 col;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) col[e] = as_bf16x8(d[e])[j];
+            for (int e = 0; e < ROWS; ++e) w[e] = d[e];
+            if (s + 2 < steps) load_wide(s + 2);
+            if constexpr (sizeof(T) == 2) {
+                bf16x8 low[RB][3];
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) acc[b][j] = mfma_16x16x32(as_bf16x8(terms[b][k]), col, acc[b][j]);
+                    for (int k = 0; k < 3; ++k)
+                        low[b][k] = as_bf16x8(lds.terms[(b * 3 + k) * 2 * kChunk + (s * 4 + q) * 16 + x]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    bf16x8 col;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) col[e] = as_bf16x8(w[e])[j];
+#pragma unroll
+                    for (int b = 0; b < RB; ++b)
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) acc[b][j] = mfma_16x16x32(low[b][k], col, acc[b][j]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < ROWS; ++e) {
+                    const f32x4 col = __builtin_bit_cast(f32x4, w[e]);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        const float low = lds.low[s * kGradRows + 4 * e + q][16 * b + x];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[b][j] = mfma_16x16x4_f32(low, col[j], acc[b][j]);
+                    }
+                }
             }
-        } else {
-            const f32x4 v = __builtin_bit_cast(f32x4, d[0]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int b = 0; b < RB; ++b) acc[b][j] = mfma_16x16x4_f32(low[b][0], v[j], acc[b][j]);
         }
-    }
-    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    __syncthreads();
+    if (pair == 1)
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int j = 0; j < E; ++j) lds.sum[wave & 1][b][j][lane] = acc[b][j];
+    __syncthreads();
+    if (pair == 1 || !any) return;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[b][j] += lds.sum[wave][b][j][lane];
     const int slot = t.slot >= 0 ? v.slot0[t.adapter] + t.slot : -1;
     if (slot >= g.slots || (t.slot >= 0 && slot < 0)) return;  // not of a plan that this library made
     float *out = slot >= 0 ? g.part + slot * (int64_t)r * W : g.out + t.adapter * (int64_t)r * W;
@@ -567,12 +763,14 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
 template <typename T, int RB>
 __global__ __launch_bounds__(256) void pool_grad_kernel(PoolParams pa, PoolGradParams ga, PoolParams pb,
                                                         PoolGradParams gb) {
+    __shared__ GradLds<T, RB> lds;
+    const PlanView v = plan_view(const_cast<int *>(pa.plan), pa.T, pa.L);
     Tile t;
-    if (!tile_of(pa, true, blockIdx.x, t) || t.adapter < 0) return;
+    if (!tile_of(pa, v, true, blockIdx.x, t) || t.adapter < 0) return;
     if ((int)blockIdx.y < ga.blocks)
-        grad_chunk<T, RB>(ga, pa, t, blockIdx.y);
+        grad_chunk<T, RB>(ga, pa, v, t, blockIdx.y, lds);
     else
-        grad_chunk<T, RB>(gb, pb, t, blockIdx.y - ga.blocks);
+        grad_chunk<T, RB>(gb, pb, v, t, blockIdx.y - ga.blocks, lds);
 }
 
 // Adapters of several chunks: the partial sums in order, times the scale;
@@ -624,8 +822,11 @@ hipError_t down_t(const PoolParams &p, hipStream_t s) {
 }
 template <typename T, bool ROWMAJOR>
 hipError_t up_t(const PoolParams &p, hipStream_t s) {
-    const int64_t blocks = ((int64_t)p.wide + 255) / 256;
-    const dim3 grid((unsigned)most_tiles(p.T, p.L, kRows), (unsigned)std::min<int64_t>(blocks, 32768)), block(256);
+    // enough workgroups for three a CU, each of as many steps as that leaves it
+    const int64_t tiles = most_tiles(p.T, p.L, kRows), blocks = ((int64_t)p.wide + 4 * kUpStep - 1) / (4 * kUpStep);
+    const int64_t want = std::max<int64_t>((3 * (int64_t)device_cu_count() + tiles - 1) / tiles, 1);
+    const int64_t turns = std::max<int64_t>(blocks / std::min(want, blocks), 1);
+    const dim3 grid((unsigned)tiles, (unsigned)((blocks + turns - 1) / turns)), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
         case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
@@ -659,7 +860,7 @@ size_t pool_plan_bytes(int T, int L) { return (size_t)plan_words(T, L) * sizeof(
 
 hipError_t launch_pool_plan(const int *index, int T, int L, int *plan, hipStream_t s) {
     const size_t lds = (size_t)(kPlanWaves * (L + 1) + 3 * (L + 2)) * sizeof(int);
-    hipLaunchKernelGGL(pool_plan_kernel, dim3(1), dim3(1024), lds, s, index, T, L, plan);
+    hipLaunchKernelGGL(pool_plan_kernel, dim3(1), dim3(1024), lds, s, index, T, L, 32 - __builtin_clz(L), plan);
     return hipGetLastError();
 }
 
@@ -712,7 +913,7 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
     PoolGradParams ga{}, gb{};
     float *part = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
     const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
-    const int cols = bf ? 512 : 256;
+    const int cols = bf ? 256 : 128;
     ga.out = c.da;
     ga.slots = gb.slots = (int)grad_slots(c.T);
     ga.part = part;
