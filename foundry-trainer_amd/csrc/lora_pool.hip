@@ -67,130 +67,124 @@ __host__ __device__ inline PlanView plan_view(int *p, int64_t T, int64_t L) {
     return v;
 }
 
+// Inclusive sum over the lanes before and at this one.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
+    return x;
+}
+
 // One workgroup.  Wave w holds the w-th sixteenth of the tokens; hist[w][a]
 // first counts its tokens of adapter a (a = L: none), then holds where in
 // `token` they begin.  The lanes of a wave that hold the same adapter find each
 // other by one ballot per bit of its number: 64 tokens of 48 adapters took 5 us
-// by one ballot per adapter, and the whole plan 11.5 us.
+// by one ballot per adapter.  Latency-bound: the index is read once, into LDS
+// where it fits, and the sums over adapters are one wave's.
+constexpr int kPlanKept = 8192;
+__host__ __device__ inline bool plan_keeps(int T, int L) { return T <= kPlanKept && L <= 1024; }
+__host__ __device__ inline int plan_lds_words(int T, int L) {
+    return kPlanWaves * (L + 1) + 3 * (L + 2) + (plan_keeps(T, L) ? T : 0);
+}
+
 __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T, int L, int bits, int *plan) {
-    extern __shared__ int hist[];  // [kPlanWaves][L + 1], then [3][L + 2]: rows, tiles and chunks before adapter a
-    __shared__ int carry[kPlanWaves][4], total[4];
+    extern __shared__ int hist[];  // [kPlanWaves][L + 1], [3][L + 2]: rows of a, tiles and chunks before it; the index
+    __shared__ int total[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, A = L + 1;
-    int *rows0 = hist + kPlanWaves * A, *tiles0 = rows0 + L + 2, *chunks0 = tiles0 + L + 2;
+    int *rows = hist + kPlanWaves * A, *tiles0 = rows + L + 2, *chunks0 = tiles0 + L + 2, *idx = chunks0 + L + 2;
     const PlanView v = plan_view(plan, T, L);
-    constexpr int kKept = 8;  // of a lane's adapters stay in registers
     const int64_t share = (((int64_t)T + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
     const int64_t t0 = wave * share, t1 = std::min<int64_t>(T, t0 + share);
-    auto adapter_of = [&](int64_t t) {
-        const int a = t < t1 ? index[t] : 0;
-        return t >= t1 ? -1 : (a < 0 || a >= L ? L : a);
-    };
-    int kept[kKept];
+    const bool kept = plan_keeps(T, L);
+    if (kept)
 #pragma unroll
-    for (int k = 0; k < kKept; ++k) kept[k] = adapter_of(t0 + 64 * k + lane);
+        for (int k = 0; k < kPlanKept / 1024; ++k)
+            if (k * 1024 + tid < T) idx[k * 1024 + tid] = index[k * 1024 + tid];
     for (int i = tid; i < kPlanWaves * A; i += 1024) hist[i] = 0;
     __syncthreads();
+    auto adapter_of = [&](int64_t t) {
+        if (t >= t1) return -1;
+        const int a = kept ? idx[t] : index[t];
+        return a < 0 || a >= L ? L : a;
+    };
     // lanes that hold the same adapter as this one
     auto peers = [&](int a) {
         uint64_t same = __ballot(a >= 0);
+        const int one = __builtin_amdgcn_readfirstlane(a);
+        if (__ballot(a == one) == same) return same;  // a whole request's
+#pragma unroll 1
         for (int b = 0; b < bits; ++b) {
             const uint64_t set = __ballot(a >> b & 1);
             same &= a >> b & 1 ? set : ~set;
         }
         return same;
     };
-    auto first_pass = [&](int a) {
+    int ahead = adapter_of(t0 + lane);
+#pragma unroll 1
+    for (int64_t t = t0; t < t1; t += 64) {
+        const int a = ahead;
+        ahead = adapter_of(t + 64 + lane);
         const uint64_t same = peers(a);
         if (a >= 0 && lane == __builtin_ctzll(same)) hist[wave * A + a] += __popcll(same);
-    };
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int tiles = 0, chunks = 0, slots = 0;  // before these 64 adapters
+#pragma unroll 1
+        for (int a0 = 0; a0 < A; a0 += 64) {
+            const int a = a0 + lane;
+            int n = 0;
+            if (a < A)
 #pragma unroll
-    for (int k = 0; k < kKept; ++k)
-        if (t0 + 64 * k < t1) first_pass(kept[k]);
-    for (int64_t t = t0 + 64 * kKept; t < t1; t += 64) first_pass(adapter_of(t + lane));
-    __syncthreads();
-    // exclusive sums over adapters of rows, tiles, chunks and partial slots:
-    // thread i holds the E adapters from i * E on
-    const int E = (A + 1023) / 1024;
-    int own[4] = {0, 0, 0, 0};
-    auto add = [&](int a, int s[4]) {
-        int n = 0;
-        for (int w = 0; w < kPlanWaves; ++w) n += hist[w * A + a];
-        const int c = a < L ? (n + kChunk - 1) / kChunk : 0;
-        s[0] += n;
-        s[1] += (n + kRows - 1) / kRows;
-        s[2] += c;
-        s[3] += c > 1 ? c : 0;
-        return n;
-    };
-    for (int e = 0; e < E; ++e)
-        if (tid * E + e < A) add(tid * E + e, own);
-    int before[4];
-    for (int k = 0; k < 4; ++k) {
-        int s = own[k];
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(s, d, 64);
-            if (lane >= d) s += o;
+                for (int w = 0; w < kPlanWaves; ++w) n += hist[w * A + a];
+            const int nt = (n + kRows - 1) / kRows, nc = a < L ? (n + kChunk - 1) / kChunk : 0, ns = nc > 1 ? nc : 0;
+            const int st = wave_scan(nt), sc = wave_scan(nc), ss = wave_scan(ns);
+            if (a < A) {
+                const int tile0 = tiles + st - nt;
+                rows[a] = n;
+                tiles0[a] = tile0;
+                chunks0[a] = chunks + sc - nc;
+                int at = tile0 * kRows;
+#pragma unroll
+                for (int w = 0; w < kPlanWaves; ++w) {
+                    const int c = hist[w * A + a];
+                    hist[w * A + a] = at;
+                    at += c;
+                }
+                if (a < L) {
+                    v.count[a] = n;
+                    v.slot0[a] = ns ? slots + ss - ns : -1;
+                }
+            }
+            tiles += __builtin_amdgcn_readlane(st, 63);
+            chunks += __builtin_amdgcn_readlane(sc, 63);
+            slots += __builtin_amdgcn_readlane(ss, 63);
         }
-        if (lane == 63) carry[wave][k] = s;
-        before[k] = s - own[k];
+        if (lane == 0) {
+            total[0] = tiles;
+            total[1] = chunks0[A] = chunks;
+            *reinterpret_cast<u32x4 *>(v.head) = u32x4{(uint32_t)tiles, (uint32_t)chunks, (uint32_t)T, (uint32_t)L};
+        }
+    } else {
+        ahead = adapter_of(t0 + lane);
     }
     __syncthreads();
-    for (int k = 0; k < 4; ++k)
-        for (int w = 0; w < wave; ++w) before[k] += carry[w][k];
-    for (int e = 0; e < E; ++e) {
-        const int a = tid * E + e;
-        if (a >= A) break;
-        rows0[a] = before[0];
-        tiles0[a] = before[1];
-        chunks0[a] = before[2];
-        const int slot0 = before[3];
-        int at = before[1] * kRows;
-        for (int w = 0; w < kPlanWaves; ++w) {
-            const int n = hist[w * A + a];
-            hist[w * A + a] = at;
-            at += n;
-        }
-        const int n = at - before[1] * kRows, c = a < L ? (n + kChunk - 1) / kChunk : 0;
-        before[0] += n;
-        before[1] += (n + kRows - 1) / kRows;
-        before[2] += c;
-        before[3] += c > 1 ? c : 0;
-        if (a < L) {
-            v.count[a] = n;
-            v.slot0[a] = c > 1 ? slot0 : -1;
-        } else {
-            rows0[A] = before[0];
-            tiles0[A] = before[1];
-            chunks0[A] = before[2];
-            total[0] = before[1];
-            total[1] = before[2];
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        v.head[0] = total[0];
-        v.head[1] = total[1];
-        v.head[2] = T;
-        v.head[3] = L;
-    }
-    auto second_pass = [&](int a, int64_t t) {
+    if (wave == 0) ahead = adapter_of(t0 + lane);
+#pragma unroll 1
+    for (int64_t t = t0; t < t1; t += 64) {
+        const int a = ahead;
+        ahead = adapter_of(t + 64 + lane);
         const uint64_t same = peers(a);
-        if (a < 0) return;
-        const int at = hist[wave * A + a];
-        v.token[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)t;
-        if (lane == __builtin_ctzll(same)) hist[wave * A + a] = at + __popcll(same);
-    };
-#pragma unroll
-    for (int k = 0; k < kKept; ++k)
-        if (t0 + 64 * k < t1) {
-            second_pass(kept[k], t0 + 64 * k + lane);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (a >= 0) {
+            const int at = hist[wave * A + a];
+            v.token[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)t + lane;
+            if (lane == __builtin_ctzll(same)) hist[wave * A + a] = at + __popcll(same);
         }
-    for (int64_t t = t0 + 64 * kKept; t < t1; t += 64) {
-        second_pass(adapter_of(t + lane), t + lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    auto find = [&](const int *first, int i) {  // the adapter a with first[a] <= i < first[a + 1]
+    auto find = [&](const int *first, int i) {  // the last adapter a with first[a] <= i
         int lo = 0, hi = A - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -201,12 +195,12 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
     };
     for (int i = tid; i < total[0]; i += 1024) {
         const int a = find(tiles0, i), k = i - tiles0[a];
-        v.tiles[i] = Tile{i, std::min(kRows, rows0[a + 1] - rows0[a] - k * kRows), a < L ? a : -1, 0};
+        v.tiles[i] = Tile{i, std::min(kRows, rows[a] - k * kRows), a < L ? a : -1, 0};
     }
     for (int i = tid; i < total[1]; i += 1024) {
         const int a = find(chunks0, i), k = i - chunks0[a];
-        v.chunks[i] = Tile{tiles0[a] + k * (kChunk / kRows), std::min(kChunk, rows0[a + 1] - rows0[a] - k * kChunk), a,
-                           chunks0[a + 1] - chunks0[a] > 1 ? k : -1};
+        v.chunks[i] = Tile{tiles0[a] + k * (kChunk / kRows), std::min(kChunk, rows[a] - k * kChunk), a,
+                           rows[a] > kChunk ? k : -1};
     }
 }
 
@@ -321,8 +315,7 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TE
 // v = B^T dy (B [wide][r])
 // ---------------------------------------------------------------------------
 // D[rank][token]: the factor is the A operand, the tokens' rows the B operand.
-// A wave takes every fourth 128-byte step of the range; a lane's 32 bytes of a
-// row are two operands.
+// A wave takes every fourth 128-byte step of the range, two operands a lane.
 template <typename T, int RB, bool ROWMAJOR>
 __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), STEP = 8 * E;
@@ -353,14 +346,14 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int64_t s = s0 + wave; s < s1; s += 4) {
-        const int64_t c = s * STEP + 2 * E * q;
-        u32x4 f[RB][2], d[4][2];
+    u32x4 f[RB][2], d[4][2];
+    auto load = [&](int64_t s) {
+        const int64_t c = s * STEP + E * q;  // its loads h: columns c + 4 E h, 64 contiguous bytes a row
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) d[i][h] = load16(rows[i], c + E * h, W);
+                for (int h = 0; h < 2; ++h) d[i][h] = load16(rows[i], c + 4 * E * h, W);
             }
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -368,25 +361,39 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if constexpr (ROWMAJOR) {
-                    f[b][h] = i < r ? load16(factor + (int64_t)i * W, c + E * h, W) : u32x4{0, 0, 0, 0};
+                    f[b][h] = i < r ? load16(factor + (int64_t)i * W, c + 4 * E * h, W) : u32x4{0, 0, 0, 0};
                 } else {
                     T w[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const int64_t m = c + E * h + e;
+                        const int64_t m = c + 4 * E * h + e;
                         w[e] = i < r && m < W ? factor[m * r + i] : (T)0.f;
                     }
                     __builtin_memcpy(&f[b][h], w, 16);
                 }
             }
         }
+    };
+    int64_t s = s0 + wave;
+    if (s < s1) load(s);
+    while (s < s1) {
+        u32x4 fc[RB][2], dc[4][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) fc[b][h] = f[b][h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dc[i][h] = d[i][h];
+        }
+        s += 4;
+        if (s < s1) load(s);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) acc[b][i] = mfma16<T>(f[b][h], d[i][h], acc[b][i]);
+                    for (int h = 0; h < 2; ++h) acc[b][i] = mfma16<T>(fc[b][h], dc[i][h], acc[b][i]);
             }
     }
 #pragma unroll
@@ -412,8 +419,9 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 // dx += s A^T v (A [r][wide])
 // ---------------------------------------------------------------------------
 // D[column][token]: a wave's step is 64 columns in four products; row 4 q + e of
-// product j is column 16 q + 4 j + e, so that a lane ends with 16 consecutive
-// columns of its token.  The rows of y and the factor of the wave's next step are
+// product j is column 32 (j / 2) + 8 q + 4 (j % 2) + e (f32: 16 j + 4 q + e), so
+// that a lane ends with 16-byte runs of its token's row, the four lanes of a row
+// with 64 bytes side by side.  The rows of y and the factor of the wave's next step are
 // loaded before this step's products.
 constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
@@ -446,6 +454,9 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     const int64_t step = (int64_t)gridDim.y * 4 * kUpStep;
     int64_t c0 = ((int64_t)blockIdx.y * 4 + wave) * kUpStep;
 
+    constexpr int RUN = 4 * E;  // columns of one load of the row's four lanes
+    // column of row m of product j, and the first of the lane's load n
+    auto column = [](int j, int m) { return sizeof(T) == 2 ? 32 * (j >> 1) + 8 * (m >> 2) + 4 * (j & 1) + (m & 3) : 16 * j + m; };
     u32x4 y[4][NY];
     u32x4 f[ROWMAJOR ? 4 : 1][RB];  // ROWMAJOR: the four products' operands
     u32x4 g[ROWMAJOR ? 1 : RB][ROWMAJOR ? 1 : 8 / E * 2];  // else rows as they lie, to be staged
@@ -454,14 +465,14 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
 #pragma unroll
-                for (int n = 0; n < NY; ++n) y[i][n] = load16(out[i], at + 16 * q + E * n, W);
+                for (int n = 0; n < NY; ++n) y[i][n] = load16(out[i], at + RUN * n + E * q, W);
             }
     };
     auto load_factor = [&](int64_t at) {
         if constexpr (ROWMAJOR) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int64_t c = at + 16 * (x >> 2) + 4 * j + (x & 3);
+                const int64_t c = at + column(j, x);
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
@@ -488,6 +499,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 #pragma unroll
         for (int b = 0; b < RB; ++b) s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (lrow < t.rows)
+#pragma unroll 4
             for (int k = 0; k < p.splits; ++k)
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
@@ -545,16 +557,16 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     if constexpr (sizeof(T) == 2) {
-                        // lane 4 e + k of 16 points at row e, column 16 k + 4 j; lane m receives column
-                        // 16 (m / 4) + 4 j + m % 4 of the four rows
-                        const uint32_t at = (16 * b + 8 * (q & 1) + (x >> 2)) * PITCH + (16 * (x & 3) + 4 * j) * 2;
+                        // lane 4 e + k of 16 points at row e, the column of product row 4 k; lane m
+                        // receives the column of product row m in the four rows
+                        const uint32_t at = (16 * b + 8 * (q & 1) + (x >> 2)) * PITCH + column(j, 4 * (x & 3)) * 2;
                         fc[j][b] = as_u32x4(lds_read_col_frag(mine, at, at + 4 * PITCH));
                     } else {
                         const float *src = reinterpret_cast<const float *>(mine);
                         f32x4 w;
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            w[e] = src[(16 * b + 4 * q + e) * (PITCH / 4) + 16 * (x >> 2) + 4 * j + (x & 3)];
+                            w[e] = src[(16 * b + 4 * q + e) * (PITCH / 4) + column(j, x)];
                         fc[j][b] = __builtin_bit_cast(u32x4, w);
                     }
                 }
@@ -564,7 +576,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
-        const int64_t c = c0 + 16 * q;
+        const int64_t c = c0 + E * q;
         c0 += step;
         if (c0 < W) {
             load_y(c0);
@@ -580,7 +592,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 #pragma unroll
                 for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b][i], acc[j]);
             }
-            if (16 * i + x >= t.rows || c >= W) continue;
+            if (16 * i + x >= t.rows) continue;
 #pragma unroll
             for (int n = 0; n < NY; ++n) {
                 if constexpr (sizeof(T) == 2) {
@@ -588,9 +600,9 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                     bf16x8 o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[e] = f32_to_bf16((float)old[e] + acc[2 * n + e / 4][e % 4]);
-                    store16(out[i], c + 8 * n, W, as_u32x4(o));
+                    store16(out[i], c + RUN * n, W, as_u32x4(o));
                 } else {
-                    store16(out[i], c + 4 * n, W,
+                    store16(out[i], c + RUN * n, W,
                             __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, yc[i][n]) + acc[n]));
                 }
             }
@@ -774,23 +786,35 @@ __global__ __launch_bounds__(256) void pool_grad_kernel(PoolParams pa, PoolGradP
 }
 
 // Adapters of several chunks: the partial sums in order, times the scale;
-// adapters without tokens: zeros.  grid (adapters, columns of 1024 elements).
+// adapters without tokens: zeros.  grid (adapters, groups of 1024 elements, dA or dB).
 __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGradParams ga, PoolGradParams gb,
                                                           int64_t na, int64_t nb) {
     const int a = blockIdx.x;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
-    if (v.head[2] != p.T || v.head[3] != p.L) return;
     const int n = v.count[a], first = v.slot0[a], chunks = (n + kChunk - 1) / kChunk;
-    if (chunks == 1) return;
+    if (v.head[2] != p.T || v.head[3] != p.L || chunks == 1) return;
     if (chunks > 1 && (first < 0 || first > ga.slots - chunks)) return;
     const float scale = p.scale[a];
-    for (int64_t e = (int64_t)blockIdx.y * 256 + threadIdx.x; e < na + nb; e += (int64_t)gridDim.y * 256) {
-        const bool is_a = e < na;
-        const int64_t at = is_a ? e : e - na, size = is_a ? na : nb;
-        float s = 0.f;
-        for (int k = 0; k < chunks; ++k) s += (is_a ? ga.part : gb.part)[(first + k) * size + at];
-        (is_a ? ga.out : gb.out)[a * size + at] = chunks ? s * scale : 0.f;
+    const int64_t size = blockIdx.z ? nb : na;
+    const float *part = (blockIdx.z ? gb.part : ga.part) + first * size;
+    float *out = (blockIdx.z ? gb.out : ga.out) + a * size;
+    for (int64_t e = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4; e < size; e += (int64_t)gridDim.y * 1024) {
+        const int left = (int)std::min<int64_t>(4, size - e);
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < chunks; ++k) s += load_f4(part + k * size + e, left);
+        store_f4(out + e, left, chunks ? s * scale : s);
     }
+}
+
+// u or v: the parts' sum, where no pool_up of it makes that.
+__global__ __launch_bounds__(256) void pool_sum_kernel(const float *low, int splits, int64_t n, float *out) {
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int left = (int)std::min<int64_t>(4, n - e);
+    if (left <= 0) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; ++k) s += load_f4(low + k * n + e, left);
+    store_f4(out + e, left, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -800,7 +824,7 @@ __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGrad
 // under 256 columns.
 int down_splits(int T, int L, int W) {
     const int64_t tiles = std::max<int64_t>(1, most_tiles(T, L, kRows));
-    const int64_t want = (2 * (int64_t)device_cu_count() + tiles - 1) / tiles;
+    const int64_t want = ((int64_t)device_cu_count() + tiles - 1) / tiles;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), W / 256));
 }
 // Partial gradients: chunks of adapters with more than one, at most two for each full one
@@ -822,10 +846,9 @@ hipError_t down_t(const PoolParams &p, hipStream_t s) {
 }
 template <typename T, bool ROWMAJOR>
 hipError_t up_t(const PoolParams &p, hipStream_t s) {
-    // enough workgroups for three a CU, each of as many steps as that leaves it
+    // two steps a wave where one each would not all fit the chip at once (three workgroups a CU)
     const int64_t tiles = most_tiles(p.T, p.L, kRows), blocks = ((int64_t)p.wide + 4 * kUpStep - 1) / (4 * kUpStep);
-    const int64_t want = std::max<int64_t>((3 * (int64_t)device_cu_count() + tiles - 1) / tiles, 1);
-    const int64_t turns = std::max<int64_t>(blocks / std::min(want, blocks), 1);
+    const int64_t turns = tiles * blocks > 3 * (int64_t)device_cu_count() ? 2 : 1;
     const dim3 grid((unsigned)tiles, (unsigned)((blocks + turns - 1) / turns)), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
@@ -853,13 +876,13 @@ hipError_t grad_t(const PoolParams &pa, const PoolGradParams &ga, const PoolPara
 hipError_t prepare_pool_kernels() {
     return hipFuncSetAttribute(reinterpret_cast<const void *>(&pool_plan_kernel),
                                hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (kPlanWaves * (kPoolMaxAdapters + 1) + 3 * (kPoolMaxAdapters + 2)) * (int)sizeof(int));
+                               plan_lds_words(kPlanKept + 1, kPoolMaxAdapters) * (int)sizeof(int));
 }
 
 size_t pool_plan_bytes(int T, int L) { return (size_t)plan_words(T, L) * sizeof(int); }
 
 hipError_t launch_pool_plan(const int *index, int T, int L, int *plan, hipStream_t s) {
-    const size_t lds = (size_t)(kPlanWaves * (L + 1) + 3 * (L + 2)) * sizeof(int);
+    const size_t lds = (size_t)plan_lds_words(T, L) * sizeof(int);
     hipLaunchKernelGGL(pool_plan_kernel, dim3(1), dim3(1024), lds, s, index, T, L, 32 - __builtin_clz(L), plan);
     return hipGetLastError();
 }
@@ -870,7 +893,8 @@ size_t pool_fwd_workspace_bytes(const PoolCall &c) {
 }
 
 size_t pool_bwd_workspace_bytes(const PoolCall &c) {
-    return low_bytes(c.T, c.r, down_splits(c.T, c.L, c.M)) +
+    const int splits = down_splits(c.T, c.L, c.M);
+    return low_bytes(c.T, c.r, splits) + (splits > 1 ? low_bytes(c.T, c.r, 1) : 0) +
            align256((size_t)grad_slots(c.T) * c.r * ((size_t)c.K + c.M) * sizeof(float));
 }
 
@@ -911,7 +935,10 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
     hipError_t e = hipSuccess;
     PoolParams pa = pv, pb = pv;  // the gradients' products
     PoolGradParams ga{}, gb{};
-    float *part = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
+    // workspace: v's parts, v, the partial gradients
+    float *v = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
+    float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(v) +
+                                            (pv.splits > 1 ? low_bytes(c.T, c.r, 1) : 0));
     const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
     const int cols = bf ? 256 : 128;
     ga.out = c.da;
@@ -934,11 +961,20 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
             px.wide = c.K;
             px.y = c.dx;
             px.ldy = c.lddx;
+            px.low_out = pv.splits > 1 && c.da ? v : nullptr;
             if ((e = bf ? up_t<bf16, false>(px, s) : up_t<float, false>(px, s)) != hipSuccess) return e;
+        }
+        if (c.da && pv.splits > 1 && !c.dx) {
+            const int64_t n = (int64_t)c.T * c.r;
+            hipLaunchKernelGGL(pool_sum_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, pv.low,
+                               pv.splits, n, v);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         pa.x = c.x;
         pa.ldx = c.ldx;
         pa.wide = c.K;
+        pa.low = pv.splits > 1 ? v : pv.low;
+        pa.splits = 1;
         pb.x = c.dy;
         pb.ldx = c.lddy;
         pb.wide = c.M;
@@ -948,9 +984,9 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
             return e;
     }
     if (!c.da) return hipSuccess;
-    const int64_t per = (na + nb + 1023) / 1024;
-    hipLaunchKernelGGL(pool_reduce_kernel, dim3(c.L, (unsigned)std::min<int64_t>(per, 256)), dim3(256), 0, s, pa, ga,
-                       gb, na, nb);
+    const int64_t per = (std::max(na, nb) + 1023) / 1024;
+    hipLaunchKernelGGL(pool_reduce_kernel, dim3(c.L, (unsigned)std::min<int64_t>(per, 1024), 2), dim3(256), 0, s, pa,
+                       ga, gb, na, nb);
     return hipGetLastError();
 }
 
