@@ -1138,7 +1138,7 @@ fa_status fa_layer_norm_fwd(const fa_layer_norm_args *a, void *stream) {
 
 size_t fa_layer_norm_bwd_workspace_size(const fa_layer_norm_bwd_args *a) {
     if (!a || a->fwd.rows < 0 || a->fwd.cols < 1 || a->fwd.cols > FA_LAYER_NORM_MAX_COLS) return 0;
-    return fa::layer_norm_bwd_workspace_bytes(a->fwd.rows, a->fwd.cols);
+    return fa::layer_norm_bwd_workspace_bytes(a->fwd.rows, a->fwd.cols, a->fwd.dtype);
 }
 
 fa_status fa_layer_norm_bwd(const fa_layer_norm_bwd_args *a, void *stream) {
@@ -1154,7 +1154,7 @@ fa_status fa_layer_norm_bwd(const fa_layer_norm_bwd_args *a, void *stream) {
     if (!aligned(a->dweight, 4) || !aligned(a->dbias, 4)) return fail(FA_ERR_INVALID_ARG, "dweight/dbias misaligned");
     const bool grads = a->dweight || a->dbias;
     if (grads) {
-        const size_t need = fa::layer_norm_bwd_workspace_bytes(f->rows, f->cols);
+        const size_t need = fa::layer_norm_bwd_workspace_bytes(f->rows, f->cols, f->dtype);
         if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need)
             return fail(FA_ERR_INVALID_ARG, "workspace is NULL, not 256-byte aligned, or smaller than %zu bytes", need);
     }

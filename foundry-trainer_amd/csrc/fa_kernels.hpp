@@ -233,7 +233,7 @@ struct LayerNormParams {
     float eps;
     int G;  // waves per row, set by the launcher
 };
-size_t layer_norm_bwd_workspace_bytes(int N, int C);
+size_t layer_norm_bwd_workspace_bytes(int N, int C, int dtype);
 hipError_t launch_layer_norm_fwd(const LayerNormParams &p, int dtype, int wdtype, hipStream_t s);
 hipError_t launch_layer_norm_bwd(const LayerNormParams &p, int dtype, int wdtype, hipStream_t s);
 

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p)
 // Backward: each group takes R rows at a time and keeps its columns' sums of
 // dy * n and dy in registers; the workgroup adds its groups' in order and
 // writes one row of partial sums [2][C].
-template <typename T, typename WT, int CH, int R>
+template <typename T, typename WT, int CH, int R, bool AHEAD>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(LayerNormParams p) {
     __shared__ float red[2][kMaxWaves][2 * R];
     extern __shared__ float part[];  // [2][C], where P > 1
@@ -192,25 +192,43 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(LayerNormParams p)
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[k][j] = db[k][j] = 0.f;
     }
-    int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * P * R; base < p.N; base += (int64_t)gridDim.x * P * R, turn ^= 1) {
-        Chunk<T> x[R][CH], dy[R][CH];
-        float mean[R], rstd[R], sum[2 * R];
+    Chunk<T> xn[R][CH], dyn[R][CH];  // the next rows
+    float meann[R], rstdn[R];
+    auto load_rows = [&](int64_t base) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int64_t row = base + group * R + i;
             const bool live = row < p.N;
             const T *xr = static_cast<const T *>(p.x) + row * p.ldx;
             const T *yr = static_cast<const T *>(p.dy) + row * p.lddy;
-            mean[i] = live ? p.mean[row] : 0.f;
-            rstd[i] = live ? p.rstd[row] : 0.f;
 #pragma unroll
             for (int k = 0; k < CH; ++k) {
                 const int e = live ? (k * G + gw) * 512 + lane * 8 : C;
-                load_chunk(xr, e, C, x[i][k]);
-                load_chunk(yr, e, C, dy[i][k]);
+                load_chunk(xr, e, C, xn[i][k]);
+                load_chunk(yr, e, C, dyn[i][k]);
             }
+            meann[i] = live ? p.mean[row] : 0.f;
+            rstdn[i] = live ? p.rstd[row] : 0.f;
         }
+    };
+    const int64_t stride = (int64_t)gridDim.x * P * R;
+    int turn = 0;
+    if (AHEAD) load_rows((int64_t)blockIdx.x * P * R);
+    for (int64_t base = (int64_t)blockIdx.x * P * R; base < p.N; base += stride, turn ^= 1) {
+        Chunk<T> x[R][CH], dy[R][CH];
+        float mean[R], rstd[R], sum[2 * R];
+        if (!AHEAD) load_rows(base);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int k = 0; k < CH; ++k) {
+                x[i][k] = xn[i][k];
+                dy[i][k] = dyn[i][k];
+            }
+            mean[i] = meann[i];
+            rstd[i] = rstdn[i];
+        }
+        if (AHEAD && base + stride < p.N) load_rows(base + stride);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             float a = 0.f, b = 0.f;
@@ -301,6 +319,7 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float *pa
     const int64_t col = (int64_t)blockIdx.x * 64 + lane;
     float s = 0.f;
     if (col < 2 * (int64_t)C)
+#pragma unroll 8
         for (int i = wave; i < count; i += 16) s += part[i * 2 * (int64_t)C + col];
     red[wave][lane] = s;
     __syncthreads();
@@ -313,24 +332,33 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float *pa
 // Waves per row of C elements with CH chunks of 512 per wave.
 int group_waves(int C, int ch) { return (C + 512 * ch - 1) / (512 * ch); }
 
+// Rows at a time of a group of waves, and whether the next are loaded ahead:
+// what 128 VGPRs hold.
+template <typename T, int CH>
+constexpr int kBwdRows = sizeof(T) == 2 && CH == 1 ? 2 : 1;
+
 struct BwdShape {
     int ch, G, P, blocks;
 };
-BwdShape bwd_shape(int N, int C) {
+// 16 waves a workgroup, one workgroup a CU; fewer waves where the rows would not
+// reach every CU otherwise.
+BwdShape bwd_shape(int N, int C, int dtype) {
     BwdShape s{};
     s.ch = C <= 8192 ? 1 : C <= 16384 ? 2 : 4;
     s.G = group_waves(C, s.ch);
-    s.P = std::max(1, kMaxWaves / s.G);
-    const int rows = s.ch == 4 ? 1 : 2;
-    s.blocks = (int)std::min<int64_t>(device_cu_count(), ((int64_t)N + s.P * rows - 1) / (s.P * rows));
+    const int64_t rows = dtype == 0 && s.ch == 1 ? 2 : 1, cus = device_cu_count();
+    s.P = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxWaves / s.G, N / (cus * rows)));
+    s.blocks = (int)std::min<int64_t>(cus * std::max(1, 8 / (s.G * s.P)), (N + s.P * rows - 1) / (s.P * rows));
     return s;
 }
 
 template <typename T, typename WT>
 hipError_t fwd_t(LayerNormParams p, hipStream_t s) {
-    const int ch = p.C <= 2048 ? 1 : p.C <= 4096 ? 2 : 4;
+    // us: 32768 x 1024 bf16 25.6 with two chunks a wave and 8 waves a workgroup, 27.4 with 4, 30.6 with
+    // one chunk (2 waves a row); 4096 x 4096 15.6 with two chunks, 17.8 with one, 16.1 with four
+    const int ch = p.C <= 512 ? 1 : p.C <= 8192 ? 2 : 4;
     p.G = group_waves(p.C, ch);
-    const int P = std::max(1, 4 / p.G);
+    const int P = std::max(1, 8 / p.G);
     const int64_t want = ((int64_t)p.N + P - 1) / P;
     const dim3 grid((unsigned)std::min<int64_t>(want, 1 << 20)), block(64 * p.G * P);
     if (ch == 1)
@@ -344,17 +372,17 @@ hipError_t fwd_t(LayerNormParams p, hipStream_t s) {
 
 template <typename T, typename WT>
 hipError_t bwd_t(LayerNormParams p, hipStream_t s) {
-    const BwdShape sh = bwd_shape(p.N, p.C);
+    const BwdShape sh = bwd_shape(p.N, p.C, sizeof(T) == 2 ? 0 : 1);
     p.G = sh.G;
     const dim3 grid(sh.blocks), block(64 * sh.G * sh.P);
     const size_t lds = p.part && sh.P > 1 ? (size_t)p.C * 8 : 0;
     if (sh.blocks > 0) {
         if (sh.ch == 1)
-            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 1, 2>), grid, block, lds, s, p);
+            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 1, kBwdRows<T, 1>, true>), grid, block, lds, s, p);
         else if (sh.ch == 2)
-            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 2, 2>), grid, block, lds, s, p);
+            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 2, kBwdRows<T, 2>, false>), grid, block, lds, s, p);
         else
-            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 4, 1>), grid, block, lds, s, p);
+            hipLaunchKernelGGL((layer_norm_bwd_kernel<T, WT, 4, kBwdRows<T, 4>, false>), grid, block, lds, s, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -368,7 +396,9 @@ hipError_t bwd_t(LayerNormParams p, hipStream_t s) {
 
 }  // namespace
 
-size_t layer_norm_bwd_workspace_bytes(int N, int C) { return (size_t)bwd_shape(N, C).blocks * 2 * C * sizeof(float); }
+size_t layer_norm_bwd_workspace_bytes(int N, int C, int dtype) {
+    return (size_t)bwd_shape(N, C, dtype).blocks * 2 * C * sizeof(float);
+}
 
 hipError_t launch_layer_norm_fwd(const LayerNormParams &p, int dtype, int wdtype, hipStream_t s) {
     if (p.N == 0) return hipSuccess;

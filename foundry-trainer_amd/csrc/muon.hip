@@ -141,102 +141,137 @@ __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
     for (int i = threadIdx.x; i < NT * kTile; i += 256) out[i] = sum[i];
 }
 
-// T of one matrix.  Wave w < RB owns the tiles (b, w) of every product.
+// T of one matrix.  Element i of a tile in lane l is (row 4 i + l / 16, column
+// l % 16).  Of up to 2 x 2 tiles each wave owns one (one alone stays in its
+// wave's registers), of more a column of them.  Bound by the latency of the
+// products one after another (four a step, three deep): 64 matrices take the
+// time of one.
 template <int RB>
 __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
     constexpr int NT = RB * (RB + 1) / 2, ALL = RB * RB * kTile;
-    extern __shared__ double lds[];  // G, Q and T, each [RB][RB] tiles of [4][64]
-    double *G = lds, *Q = lds + ALL, *T = lds + 2 * ALL;
-    __shared__ double trace;
+    constexpr int OWN = RB <= 2 ? 1 : RB, WAVES = RB * RB / OWN;  // tiles of a wave, waves that have some
+    extern __shared__ double lds[];  // G, Q, T and H = G Q, each [RB][RB] tiles of [4][64]
+    double *G = lds, *Q = lds + ALL, *T = lds + 2 * ALL, *H = lds + 3 * ALL;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int k = 0;
     while (k + 1 < p.items && p.matrix0[k + 1] <= (int)blockIdx.x) ++k;
     const int64_t matrix = blockIdx.x - p.matrix0[k];
-    const double *part = p.gram + (p.gram0[k] + matrix * p.chunks[k] * (int64_t)(NT * kTile));
-    // element i of a tile in lane l is (row 4 i + l / 16, column l % 16)
+    const int chunks = p.chunks[k];
+    const double *part = p.gram + (p.gram0[k] + matrix * chunks * (int64_t)(NT * kTile));
     auto tile = [](double *M, int b, int c) { return M + (b * RB + c) * kTile; };
-    for (int e = threadIdx.x; e < NT * kTile; e += 256) {
-        double s = 0;
-        for (int c = 0; c < p.chunks[k]; ++c) s += part[c * (int64_t)(NT * kTile) + e];
-        int t = e / kTile, b = 0;
-        while (t >= RB - b) t -= RB - b, ++b;
-        const int c = b + t, i = e / 64 % 4, l = e & 63, row = 4 * i + l / 16, col = l % 16;
-        tile(G, b, c)[i * 64 + l] = s;
-        if (c != b) tile(G, c, b)[(col / 4) * 64 + (col % 4) * 16 + row] = s;
-    }
+    double sum[NT] = {};  // element threadIdx.x of every tile; no branch between the loads
+#pragma unroll(RB <= 2 ? 8 : 4)
+    for (int c = 0; c < chunks; ++c)
+#pragma unroll
+        for (int o = 0; o < NT; ++o) sum[o] += part[c * (int64_t)(NT * kTile) + o * kTile + threadIdx.x];
+#pragma unroll
+    for (int b = 0, o = 0; b < RB; ++b)
+#pragma unroll
+        for (int c = b; c < RB; ++c, ++o) {
+            const int row = 4 * wave + lane / 16, col = lane % 16;
+            tile(G, b, c)[threadIdx.x] = sum[o];
+            if (c != b) tile(G, c, b)[(col / 4) * 64 + (col % 4) * 16 + row] = sum[o];
+        }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double s = 0;
-        for (int b = 0; b < RB; ++b)
-            for (int d = 0; d < 16; ++d) s += tile(G, b, b)[(d / 4) * 64 + (d % 4) * 16 + d];
-        trace = s;
-    }
-    __syncthreads();
-    const double inv = 1.0 / (sqrt(trace) + p.eps);
-    for (int e = threadIdx.x; e < ALL; e += 256) {
-        const int b = e / kTile / RB, c = e / kTile % RB, i = e / 64 % 4, l = e & 63;
-        G[e] *= inv * inv;
-        T[e] = b == c && 4 * i + l / 16 == l % 16 ? 1.0 : 0.0;
-    }
-    __syncthreads();
-    // tiles (b, wave) of A B for symmetric, commuting A and B
-    auto product = [&](double *A, double *B, f64x4 *out) {
+    // the trace, in every wave: lane d < 16 RB has diagonal element d
+    double trace = 0;
+    if (lane < 16 * RB) trace = tile(G, lane / 16, lane / 16)[(lane % 16 / 4) * 64 + (lane % 4) * 16 + lane % 16];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) out[b] = f64x4{0, 0, 0, 0};
+    for (int d = 32; d; d >>= 1) trace += __shfl_xor(trace, d, 64);
+    const double norm = sqrt(trace) + p.eps, inv = 1.0 / norm;
+    const bool mine = wave < WAVES;
+    if (RB == 1 && !mine) return;  // no barrier follows
+    const int b0 = OWN == 1 ? wave / RB : 0, c0 = mine ? wave % RB : 0;  // tiles (b0 + u, c0)
+    f64x4 g[OWN], t[OWN];
+    auto diagonal = [&](int u, int i) { return b0 + u == c0 && 4 * i + lane / 16 == lane % 16; };
 #pragma unroll
-        for (int q = 0; q < RB; ++q)
+    for (int u = 0; u < OWN; ++u)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const double y = tile(B, q, wave)[t * 64 + lane];
+        for (int i = 0; i < 4; ++i) {
+            g[u][i] = mine ? tile(G, b0 + u, c0)[i * 64 + lane] * (inv * inv) : 0.0;
+            t[u][i] = diagonal(u, i) ? 1.0 : 0.0;
+        }
+    const f64x4 zero = {0, 0, 0, 0};
+    auto polynomial = [&](f64x4 (&q)[OWN]) {
 #pragma unroll
-                for (int b = 0; b < RB; ++b) out[b] = mfma_f64(tile(A, q, b)[t * 64 + lane], y, out[b]);
-            }
+        for (int u = 0; u < OWN; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[u][i] = p.c * q[u][i] + p.b * g[u][i] + (diagonal(u, i) ? p.a : 0.0);
     };
-    auto keep = [&](double *M, const f64x4 *v) {
+    if constexpr (RB == 1) {
+        auto product = [&](f64x4 x, f64x4 y) {
+            f64x4 z = zero;
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
+            for (int i = 0; i < 4; ++i) z = mfma_f64(x[i], y[i], z);
+            return z;
+        };
+        for (int step = 0; step < p.steps; ++step) {
+            f64x4 q[1] = {product(g[0], g[0])};
+            polynomial(q);
+            t[0] = product(t[0], q[0]);
+            g[0] = product(product(g[0], q[0]), q[0]);
+        }
+    } else {
+        auto keep = [&](double *M, const f64x4 (&v)[OWN]) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) tile(M, b, wave)[t * 64 + lane] = v[b][t];
-    };
-    const bool mine = wave < RB;
-    for (int step = 0; step < p.steps; ++step) {
-        f64x4 v[RB], w[RB];
-        if (mine) {
-            product(G, G, v);
+            for (int u = 0; u < OWN; ++u)
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
+                for (int i = 0; i < 4; ++i)
+                    if (mine) tile(M, b0 + u, c0)[i * 64 + lane] = v[u][i];
+        };
+        // the wave's tiles of X Y for symmetric, commuting X and Y; a single tile's in two chains
+        auto product = [&](double *X, double *Y, f64x4 (&z)[OWN]) {
+            if (!mine) return;
+            constexpr int CHAINS = OWN == 1 ? 2 : 1;
+            f64x4 w[OWN][CHAINS];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const bool diag = b == wave && 4 * t + lane / 16 == lane % 16;
-                    v[b][t] = p.c * v[b][t] + p.b * tile(G, b, wave)[t * 64 + lane] + (diag ? p.a : 0.0);
+            for (int u = 0; u < OWN; ++u)
+#pragma unroll
+                for (int h = 0; h < CHAINS; ++h) w[u][h] = zero;
+#pragma unroll
+            for (int q = 0; q < RB; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double y = tile(Y, q, c0)[i * 64 + lane];
+#pragma unroll
+                    for (int u = 0; u < OWN; ++u)
+                        w[u][i % CHAINS] = mfma_f64(tile(X, q, b0 + u)[i * 64 + lane], y, w[u][i % CHAINS]);
                 }
+#pragma unroll
+            for (int u = 0; u < OWN; ++u) z[u] = CHAINS == 2 ? w[u][0] + w[u][CHAINS - 1] : w[u][0];
+        };
+        __syncthreads();  // every wave has read its part of G unscaled
+        keep(G, g);
+        keep(T, t);
+        for (int step = 0; step < p.steps; ++step) {
+            const bool last = step + 1 == p.steps;
+            f64x4 v[OWN];
+            __syncthreads();
+            product(G, G, v);
+            polynomial(v);
             keep(Q, v);
-        }
-        __syncthreads();
-        const bool last = step + 1 == p.steps;
-        if (mine) {
-            product(T, Q, v);
-            if (!last) product(G, Q, w);
-        }
-        __syncthreads();
-        if (mine) {
-            keep(T, v);
-            if (!last) keep(G, w);
-        }
-        __syncthreads();
-        if (!last) {
-            if (mine) product(G, Q, w);
             __syncthreads();
-            if (mine) keep(G, w);
+            product(T, Q, t);
+            if (last) break;
+            product(G, Q, v);
+            keep(H, v);
             __syncthreads();
+            keep(T, t);
+            product(H, Q, g);
+            keep(G, g);
         }
     }
-    // 1 / (norm + eps) as a power of two, which u takes, and what is left, which
-    // T takes: neither leaves f32's range, whatever the gradients' scale
+    if (!mine) return;
+    // 1 / norm as a power of two, which u takes, and what is left, which T takes:
+    // neither leaves f32's range, whatever the gradients' scale
     int expo;
-    const double part_of_norm = frexp(sqrt(trace) + p.eps, &expo);
-    float *out = p.turn + (int64_t)blockIdx.x * ALL;
-    for (int e = threadIdx.x; e < ALL; e += 256) out[e] = (float)(T[e] / part_of_norm);
+    const double part_of_norm = frexp(norm, &expo);
+#pragma unroll
+    for (int u = 0; u < OWN; ++u) {
+        float *out = p.turn + (int64_t)blockIdx.x * ALL + ((b0 + u) * RB + c0) * kTile;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i * 64 + lane] = (float)(t[u][i] / part_of_norm);
+    }
     if (threadIdx.x == 0) p.expo[blockIdx.x] = -expo;
 }
 
@@ -418,7 +453,7 @@ size_t lay_out(MuonMany &p, int rb) {
 template <int RB>
 hipError_t run_rb(const MuonMany &p, int dtype, hipStream_t s) {
     const dim3 blocks(p.block0[p.items]), matrices(p.matrix0[p.items]), t(256);
-    const size_t lds = 3 * RB * RB * kTile * sizeof(double);
+    const size_t lds = (RB == 1 ? 1 : 4) * RB * RB * kTile * sizeof(double);
     hipLaunchKernelGGL((muon_gram_kernel<RB>), blocks, t, 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -435,10 +470,10 @@ hipError_t run_rb(const MuonMany &p, int dtype, hipStream_t s) {
 
 hipError_t prepare_muon_kernels() {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&muon_solve_kernel<3>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 9 * kTile * 8);
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 9 * kTile * 8);
     if (e != hipSuccess) return e;
     return hipFuncSetAttribute(reinterpret_cast<const void *>(&muon_solve_kernel<4>),
-                               hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 16 * kTile * 8);
+                               hipFuncAttributeMaxDynamicSharedMemorySize, 4 * 16 * kTile * 8);
 }
 
 int muon_row_blocks(int rows, int cols) { return (std::min(rows, cols) + 15) / 16; }
