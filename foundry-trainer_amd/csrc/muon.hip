@@ -144,8 +144,9 @@ __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
 // T of one matrix.  Element i of a tile in lane l is (row 4 i + l / 16, column
 // l % 16).  Of up to 2 x 2 tiles each wave owns one (one alone stays in its
 // wave's registers), of more a column of them.  Bound by the latency of the
-// products one after another (four a step, three deep): 64 matrices take the
-// time of one.
+// products one after another (four a step, three deep, an MFMA 64 cycles): 64
+// matrices take the time of one.  Only the tiles on and above the diagonal, mirrored
+// in LDS, would be 10 of 16 products at rank 64, but measured 52 us against 47.
 template <int RB>
 __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
     constexpr int NT = RB * (RB + 1) / 2, ALL = RB * RB * kTile;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
     const double *part = p.gram + (p.gram0[k] + matrix * chunks * (int64_t)(NT * kTile));
     auto tile = [](double *M, int b, int c) { return M + (b * RB + c) * kTile; };
     double sum[NT] = {};  // element threadIdx.x of every tile; no branch between the loads
-#pragma unroll(RB <= 2 ? 8 : 4)
+#pragma unroll 8
     for (int c = 0; c < chunks; ++c)
 #pragma unroll
         for (int o = 0; o < NT; ++o) sum[o] += part[c * (int64_t)(NT * kTile) + o * kTile + threadIdx.x];
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
         for (int step = 0; step < p.steps; ++step) {
             f64x4 q[1] = {product(g[0], g[0])};
             polynomial(q);
-            t[0] = product(t[0], q[0]);
+            t[0] = step ? product(t[0], q[0]) : q[0];
             g[0] = product(product(g[0], q[0]), q[0]);
         }
     } else {
@@ -242,7 +243,6 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
         };
         __syncthreads();  // every wave has read its part of G unscaled
         keep(G, g);
-        keep(T, t);
         for (int step = 0; step < p.steps; ++step) {
             const bool last = step + 1 == p.steps;
             f64x4 v[OWN];
@@ -251,7 +251,12 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
             polynomial(v);
             keep(Q, v);
             __syncthreads();
-            product(T, Q, t);
+            if (step) {
+                product(T, Q, t);
+            } else {
+#pragma unroll
+                for (int u = 0; u < OWN; ++u) t[u] = v[u];  // Q itself
+            }
             if (last) break;
             product(G, Q, v);
             keep(H, v);
