@@ -204,9 +204,19 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
     }
 }
 
+// Workgroups run column by column of a tile, then the next tile: those at work at
+// once hold whole rows.  (Tile by tile of a column block, a 512-byte piece of
+// every row, 6000 x 8192 took the expand product 53 us.)
+constexpr int kGridTiles = 32768;
+dim3 tile_grid(int64_t columns, int64_t tiles) {
+    return dim3((unsigned)columns, (unsigned)std::min<int64_t>(tiles, kGridTiles),
+                (unsigned)((tiles + kGridTiles - 1) / kGridTiles));
+}
+__device__ __forceinline__ int64_t grid_tile() { return (int64_t)blockIdx.z * kGridTiles + blockIdx.y; }
+
 // Tile or chunk i of the plan as the kernels trust it: nothing of it leads
 // outside the call's tensors, whatever memory the plan was given.
-__device__ __forceinline__ bool tile_of(const PoolParams &p, const PlanView &v, bool chunk, int i, Tile &t) {
+__device__ __forceinline__ bool tile_of(const PoolParams &p, const PlanView &v, bool chunk, int64_t i, Tile &t) {
     // all loads at once: the tile's place holds some word, whether or not there is such a tile
     const u32x4 head = *reinterpret_cast<const u32x4 *>(v.head);
     const u32x4 w = *reinterpret_cast<const u32x4 *>((chunk ? v.chunks : v.tiles) + i);
@@ -222,9 +232,9 @@ __device__ __forceinline__ int token_at(const PoolParams &p, const PlanView &v, 
 }
 // Its tokens, for a lane that reads row 16 i + x of a row tile in its i-th load:
 // rows past the end read the block's first (and are not written).
-__device__ __forceinline__ void tile_tokens(const PoolParams &p, const PlanView &v, int tile, int x, int (&token)[4]) {
+__device__ __forceinline__ void tile_tokens(const PoolParams &p, const PlanView &v, int64_t tile, int x, int (&token)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) token[i] = token_at(p, v, (int64_t)tile * kRows + 16 * i + x);
+    for (int i = 0; i < 4; ++i) token[i] = token_at(p, v, tile * kRows + 16 * i + x);
 }
 __device__ __forceinline__ void clamp_tokens(const Tile &t, int x, int (&token)[4]) {
 #pragma unroll
@@ -237,11 +247,12 @@ __device__ __forceinline__ void clamp_tokens(const Tile &t, int x, int (&token)[
 // ---------------------------------------------------------------------------
 // loads and operands
 // ---------------------------------------------------------------------------
-// 16 bytes from column c of a row of n elements; zero past its end.
-template <typename T>
+// 16 bytes from column c of a row of n elements; zero past its end.  FULL: they
+// all lie in the row (where a whole wave knows that, its loads need no branches).
+template <bool FULL = false, typename T>
 __device__ __forceinline__ u32x4 load16(const T *row, int64_t c, int64_t n) {
     constexpr int E = 16 / sizeof(T);
-    if (c + E <= n) return *reinterpret_cast<const u32x4_any *>(row + c);
+    if (FULL || c + E <= n) return *reinterpret_cast<const u32x4_any *>(row + c);
     T v[E] = {};
 #pragma unroll
     for (int j = 0; j < E; ++j)
@@ -262,6 +273,9 @@ __device__ __forceinline__ void store16(T *row, int64_t c, int64_t n, u32x4 w) {
 #pragma unroll
     for (int j = 0; j < E; ++j)
         if (c + j < n) row[c + j] = v[j];
+}
+__device__ __forceinline__ u32x4 zero_unless(bool keep, u32x4 v) {
+    return u32x4{keep ? v[0] : 0u, keep ? v[1] : 0u, keep ? v[2] : 0u, keep ? v[3] : 0u};
 }
 __device__ __forceinline__ f32x4 load_f4(const float *base, int left) {
     if (left >= 4) return *reinterpret_cast<const f32x4_any *>(base);
@@ -322,13 +336,15 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     __shared__ f32x4 sum[4][RB][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    const int64_t at = grid_tile();
+    if (at >= most_tiles(p.T, p.L, kRows)) return;
     int token[4];
-    tile_tokens(p, v, blockIdx.x, x, token);
+    tile_tokens(p, v, at, x, token);
     Tile t;
-    if (!tile_of(p, v, false, blockIdx.x, t)) return;
+    if (!tile_of(p, v, false, at, t)) return;
     clamp_tokens(t, x, token);
     const int r = p.r, W = p.wide;
-    const int64_t part = (int64_t)blockIdx.y * p.T;
+    const int64_t part = (int64_t)blockIdx.x * p.T;
     if (t.adapter < 0) {
         for (int i = threadIdx.x; i < t.rows * r; i += 256)
             p.low[(part + token_at(p, v, (int64_t)t.tile * kRows + i / r)) * r + i % r] = 0.f;
@@ -336,7 +352,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     }
     const int subs = (t.rows + 15) / 16;
     const int64_t steps = ((int64_t)W + STEP - 1) / STEP;
-    const int64_t s0 = steps * blockIdx.y / gridDim.y, s1 = steps * (blockIdx.y + 1) / gridDim.y;
+    const int64_t s0 = steps * blockIdx.x / gridDim.x, s1 = steps * (blockIdx.x + 1) / gridDim.x;
     const T *rows[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) rows[i] = static_cast<const T *>(p.x) + token[i] * p.ldx;
@@ -347,32 +363,38 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     u32x4 f[RB][2], d[4][2];
-    auto load = [&](int64_t s) {
+    // a factor row past the rank is the last one's again: its sums are not stored
+    auto load_step = [&](auto full, int64_t s) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
         const int64_t c = s * STEP + E * q;  // its loads h: columns c + 4 E h, 64 contiguous bytes a row
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) d[i][h] = load16(rows[i], c + 4 * E * h, W);
+                for (int h = 0; h < 2; ++h) d[i][h] = load16<FULL>(rows[i], c + 4 * E * h, W);
             }
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            const int i = 16 * b + x;
+            const int i = std::min(16 * b + x, r - 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if constexpr (ROWMAJOR) {
-                    f[b][h] = i < r ? load16(factor + (int64_t)i * W, c + 4 * E * h, W) : u32x4{0, 0, 0, 0};
+                    f[b][h] = load16<FULL>(factor + (int64_t)i * W, c + 4 * E * h, W);
                 } else {
                     T w[E];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         const int64_t m = c + 4 * E * h + e;
-                        w[e] = i < r && m < W ? factor[m * r + i] : (T)0.f;
+                        w[e] = FULL || m < W ? factor[m * r + i] : (T)0.f;
                     }
                     __builtin_memcpy(&f[b][h], w, 16);
                 }
             }
         }
+    };
+    auto load = [&](int64_t s) __attribute__((always_inline)) {
+        if ((s + 1) * STEP <= W) load_step(std::true_type{}, s);
+        else load_step(std::false_type{}, s);
     };
     int64_t s = s0 + wave;
     if (s < s1) load(s);
@@ -435,24 +457,26 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     __shared__ __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    const int64_t at = grid_tile();
+    if (at >= most_tiles(p.T, p.L, kRows)) return;
     int token[4];
-    tile_tokens(p, v, blockIdx.x, x, token);
+    tile_tokens(p, v, at, x, token);
     // four threads a row: its ranks 4 h .. of every 16, the parts in order
     const int h = threadIdx.x & 3, lrow = threadIdx.x >> 2;
-    const int ltoken = token_at(p, v, (int64_t)blockIdx.x * kRows + lrow);
+    const int ltoken = token_at(p, v, at * kRows + lrow);
     Tile t;
-    if (!tile_of(p, v, false, blockIdx.x, t)) return;
+    if (!tile_of(p, v, false, at, t)) return;
     clamp_tokens(t, x, token);
     const int r = p.r, W = p.wide, subs = (t.rows + 15) / 16;
     const bool live = t.adapter >= 0;
-    if (!live && !(p.low_out && blockIdx.y == 0)) return;
+    if (!live && !(p.low_out && blockIdx.x == 0)) return;
     const float scale = live ? p.scale[t.adapter] : 0.f;
     const T *factor = static_cast<const T *>(p.factor) + (int64_t)(live ? t.adapter : 0) * r * W;
     T *out[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = static_cast<T *>(p.y) + token[i] * p.ldy;
-    const int64_t step = (int64_t)gridDim.y * 4 * kUpStep;
-    int64_t c0 = ((int64_t)blockIdx.y * 4 + wave) * kUpStep;
+    const int64_t step = (int64_t)gridDim.x * 4 * kUpStep;
+    int64_t c0 = ((int64_t)blockIdx.x * 4 + wave) * kUpStep;
 
     constexpr int RUN = 4 * E;  // columns of one load of the row's four lanes
     // column of row m of product j, and the first of the lane's load n
@@ -460,23 +484,24 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     u32x4 y[4][NY];
     u32x4 f[ROWMAJOR ? 4 : 1][RB];  // ROWMAJOR: the four products' operands
     u32x4 g[ROWMAJOR ? 1 : RB][ROWMAJOR ? 1 : 8 / E * 2];  // else rows as they lie, to be staged
-    auto load_y = [&](int64_t at) {
+    const bool whole_rank = r == 16 * RB;
+    auto load_step = [&](auto full, int64_t col) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
 #pragma unroll
-                for (int n = 0; n < NY; ++n) y[i][n] = load16(out[i], at + RUN * n + E * q, W);
+                for (int n = 0; n < NY; ++n) y[i][n] = load16<FULL>(out[i], col + RUN * n + E * q, W);
             }
-    };
-    auto load_factor = [&](int64_t at) {
         if constexpr (ROWMAJOR) {
+            // a column past the row's end is the last one's again: its sums are not stored
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int64_t c = at + column(j, x);
+                const T *row = factor + std::min<int64_t>(col + column(j, x), W - 1) * r;
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
-                    f[j][b] = c < W ? load16(factor + c * r, k, r) : u32x4{0, 0, 0, 0};
+                    f[j][b] = load16<FULL>(row, k, r);
                 }
             }
         } else {
@@ -486,14 +511,16 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 #pragma unroll
                 for (int n = 0; n < 16 * LANES / 64; ++n) {
                     const int i = 16 * b + n * (64 / LANES) + lane / LANES;
-                    g[b][n] = i < r ? load16(factor + (int64_t)i * W, at + E * (lane % LANES), W) : u32x4{0, 0, 0, 0};
+                    const T *row = factor + (int64_t)std::min(i, r - 1) * W;
+                    g[b][n] = zero_unless(i < r, load16<FULL>(row, col + E * (lane % LANES), W));
                 }
         }
     };
-    if (live && c0 < W) {
-        load_y(c0);
-        load_factor(c0);
-    }
+    auto load = [&](int64_t col) __attribute__((always_inline)) {
+        if (col + kUpStep <= W && (!ROWMAJOR || whole_rank)) load_step(std::true_type{}, col);
+        else load_step(std::false_type{}, col);
+    };
+    if (live && c0 < W) load(c0);
     {
         f32x4 s[RB];
 #pragma unroll
@@ -506,7 +533,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                     s[b] += load_f4(p.low + ((int64_t)k * p.T + ltoken) * r + 16 * b + 4 * h, r - 16 * b - 4 * h);
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            if (p.low_out && blockIdx.y == 0 && lrow < t.rows)  // the parts' sum, for the backward
+            if (p.low_out && blockIdx.x == 0 && lrow < t.rows)  // the parts' sum, for the backward
                 store_f4(p.low_out + (int64_t)ltoken * r + 16 * b + 4 * h, r - 16 * b - 4 * h, s[b]);
             *reinterpret_cast<f32x4 *>(&lowsum[lrow][16 * b + 4 * h]) = s[b] * scale;
         }
@@ -559,8 +586,8 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                     if constexpr (sizeof(T) == 2) {
                         // lane 4 e + k of 16 points at row e, the column of product row 4 k; lane m
                         // receives the column of product row m in the four rows
-                        const uint32_t at = (16 * b + 8 * (q & 1) + (x >> 2)) * PITCH + column(j, 4 * (x & 3)) * 2;
-                        fc[j][b] = as_u32x4(lds_read_col_frag(mine, at, at + 4 * PITCH));
+                        const uint32_t src = (16 * b + 8 * (q & 1) + (x >> 2)) * PITCH + column(j, 4 * (x & 3)) * 2;
+                        fc[j][b] = as_u32x4(lds_read_col_frag(mine, src, src + 4 * PITCH));
                     } else {
                         const float *src = reinterpret_cast<const float *>(mine);
                         f32x4 w;
@@ -578,10 +605,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
             for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
         const int64_t c = c0 + E * q;
         c0 += step;
-        if (c0 < W) {
-            load_y(c0);
-            load_factor(c0);
-        }
+        if (c0 < W) load(c0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i >= subs) continue;
@@ -644,19 +668,26 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
     const int64_t base = ((int64_t)block * 2 + (wave & 1)) * 16 * E, c = base + E * x;
     const int steps = (t.rows + kGradRows - 1) / kGradRows;
     {
+        // rows past the end: the first one's token, negative (~token)
         const int i = threadIdx.x;
-        const int token = i < t.rows ? token_at(p, v, (int64_t)t.tile * kRows + i) : -1;
-        lds.token[i] = token;
+        const int token = token_at(p, v, (int64_t)t.tile * kRows + (i < t.rows ? i : 0));
+        lds.token[i] = i < t.rows ? token : ~token;
     }
     __syncthreads();
     u32x4 d[ROWS];
     // bf16: rows 8 q + e of the step; f32: rows 4 e + q
-    auto load_wide = [&](int s) {
+    auto load_rows = [&](auto full, int s) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
 #pragma unroll
         for (int e = 0; e < ROWS; ++e) {
             const int token = lds.token[s * kGradRows + (sizeof(T) == 2 ? 8 * q + e : 4 * e + q)];
-            d[e] = token >= 0 ? load16(static_cast<const T *>(p.x) + token * p.ldx, c, W) : u32x4{0, 0, 0, 0};
+            const T *row = static_cast<const T *>(p.x) + (token < 0 ? ~token : token) * p.ldx;
+            d[e] = zero_unless(token >= 0, load16<FULL>(row, c, W));
         }
+    };
+    auto load_wide = [&](int s) __attribute__((always_inline)) {
+        if (base + 16 * E <= W) load_rows(std::true_type{}, s);
+        else load_rows(std::false_type{}, s);
     };
     const bool any = base < W;
     if (any && pair < steps) load_wide(pair);
@@ -778,11 +809,12 @@ __global__ __launch_bounds__(256) void pool_grad_kernel(PoolParams pa, PoolGradP
     __shared__ GradLds<T, RB> lds;
     const PlanView v = plan_view(const_cast<int *>(pa.plan), pa.T, pa.L);
     Tile t;
-    if (!tile_of(pa, v, true, blockIdx.x, t) || t.adapter < 0) return;
-    if ((int)blockIdx.y < ga.blocks)
-        grad_chunk<T, RB>(ga, pa, v, t, blockIdx.y, lds);
+    const int64_t at = grid_tile();
+    if (at >= most_tiles(pa.T, pa.L, kChunk) || !tile_of(pa, v, true, at, t) || t.adapter < 0) return;
+    if ((int)blockIdx.x < ga.blocks)
+        grad_chunk<T, RB>(ga, pa, v, t, blockIdx.x, lds);
     else
-        grad_chunk<T, RB>(gb, pb, v, t, blockIdx.y - ga.blocks, lds);
+        grad_chunk<T, RB>(gb, pb, v, t, blockIdx.x - ga.blocks, lds);
 }
 
 // Adapters of several chunks: the partial sums in order, times the scale;
@@ -820,12 +852,16 @@ __global__ __launch_bounds__(256) void pool_sum_kernel(const float *low, int spl
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Ranges of the wide axis: enough workgroups for two rounds of the chip, none
-// under 256 columns.
+// Ranges of the wide axis: about a workgroup a CU, a power of two so that the
+// waves' steps divide evenly, none under 256 columns.  us of down + up, 6000 x 2048
+// -> 8192 rank 32: one range 64, two 60, three 64, four 61, eight 65; 4096 x 4096
+// rank 16: two 33, four 30, eight 30.
 int down_splits(int T, int L, int W) {
     const int64_t tiles = std::max<int64_t>(1, most_tiles(T, L, kRows));
-    const int64_t want = ((int64_t)device_cu_count() + tiles - 1) / tiles;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), W / 256));
+    const int64_t want = ((int64_t)device_cu_count() * 4 / 3 + tiles - 1) / tiles;
+    int64_t splits = 1;
+    while (2 * splits <= std::min<int64_t>(std::min<int64_t>(want, 64), W / 256)) splits *= 2;
+    return (int)splits;
 }
 // Partial gradients: chunks of adapters with more than one, at most two for each full one
 int64_t grad_slots(int T) { return 2 * ((int64_t)T / kChunk); }
@@ -835,7 +871,7 @@ size_t low_bytes(int T, int r, int splits) { return align256((size_t)splits * T 
 
 template <typename T, bool ROWMAJOR>
 hipError_t down_t(const PoolParams &p, hipStream_t s) {
-    const dim3 grid((unsigned)most_tiles(p.T, p.L, kRows), p.splits), block(256);
+    const dim3 grid = tile_grid(p.splits, most_tiles(p.T, p.L, kRows)), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_down_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
         case 2: hipLaunchKernelGGL((pool_down_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
@@ -849,7 +885,7 @@ hipError_t up_t(const PoolParams &p, hipStream_t s) {
     // two steps a wave where one each would not all fit the chip at once (three workgroups a CU)
     const int64_t tiles = most_tiles(p.T, p.L, kRows), blocks = ((int64_t)p.wide + 4 * kUpStep - 1) / (4 * kUpStep);
     const int64_t turns = tiles * blocks > 3 * (int64_t)device_cu_count() ? 2 : 1;
-    const dim3 grid((unsigned)tiles, (unsigned)((blocks + turns - 1) / turns)), block(256);
+    const dim3 grid = tile_grid((blocks + turns - 1) / turns, tiles), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
         case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
@@ -861,7 +897,7 @@ hipError_t up_t(const PoolParams &p, hipStream_t s) {
 template <typename T>
 hipError_t grad_t(const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb, const PoolGradParams &gb,
                   hipStream_t s) {
-    const dim3 grid((unsigned)most_tiles(pa.T, pa.L, kChunk), ga.blocks + gb.blocks), block(256);
+    const dim3 grid = tile_grid(ga.blocks + gb.blocks, most_tiles(pa.T, pa.L, kChunk)), block(256);
     switch ((pa.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_grad_kernel<T, 1>), grid, block, 0, s, pa, ga, pb, gb); break;
         case 2: hipLaunchKernelGGL((pool_grad_kernel<T, 2>), grid, block, 0, s, pa, ga, pb, gb); break;

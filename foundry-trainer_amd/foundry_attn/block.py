@@ -1112,6 +1112,11 @@ class DoubleBlockLoRA:
         """One AdamW step of every LoRA factor (adamw_step, lib.rs:477-510),
         all factors in one fa_adamw_step_many call."""
         self.step_count += 1
+        adamw_step_many(self._factor_states(grads), self.step_count, lr, betas, eps)
+        self.refresh_adapters()
+
+    def _factor_states(self, grads):
+        """(factor, gradient, first moment, second moment) of every LoRA factor."""
         items = []
         for (name, t), g in grads.items():
             if t == "x":
@@ -1120,7 +1125,13 @@ class DoubleBlockLoRA:
             w = self.w[name]
             items.append((w.lora_a[t], da, w.m[f"{t}.a"], w.v[f"{t}.a"]))
             items.append((w.lora_b[t], db, w.m[f"{t}.b"], w.v[f"{t}.b"]))
-        adamw_step_many(items, self.step_count, lr, betas, eps)
+        return items
+
+    def apply_muon(self, grads, lr: float = 0.02, **kw) -> None:
+        """One orthogonalised step of every LoRA factor (muon_step_many, its
+        options in kw) instead of AdamW's; the momentum is AdamW's first
+        moment, so a run keeps to one of the two."""
+        muon_step_many([it[:3] for it in self._factor_states(grads)], lr=lr, **kw)
         self.refresh_adapters()
 
     def train_step(self, x, dy, lr: float = 1e-3, want_dx: bool = False):
@@ -1400,13 +1411,22 @@ class SingleBlockLoRA:
 
     def apply_adamw(self, grads, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8) -> None:
         self.step_count += 1
+        adamw_step_many(self._factor_states(grads), self.step_count, lr, betas, eps)
+        self.refresh_adapters()
+
+    def _factor_states(self, grads):
+        """(factor, gradient, first moment, second moment) of every LoRA factor."""
         w = self.w
         items = []
         for t in SINGLE_LORA_TARGETS:
             da, db = grads[t]
             items.append((w.lora_a[t], da, w.m[f"{t}.a"], w.v[f"{t}.a"]))
             items.append((w.lora_b[t], db, w.m[f"{t}.b"], w.v[f"{t}.b"]))
-        adamw_step_many(items, self.step_count, lr, betas, eps)
+        return items
+
+    def apply_muon(self, grads, lr: float = 0.02, **kw) -> None:
+        """DoubleBlockLoRA.apply_muon of this block's factors."""
+        muon_step_many([it[:3] for it in self._factor_states(grads)], lr=lr, **kw)
         self.refresh_adapters()
 
     def train_step(self, x, dy, lr: float = 1e-3, want_dx: bool = True):

@@ -48,6 +48,9 @@ class DoubleStage:
     def apply_adamw(self, grads, lr: float) -> None:
         self.block.apply_adamw(grads, lr)
 
+    def apply_muon(self, grads, lr: float, **kw) -> None:
+        self.block.apply_muon(grads, lr, **kw)
+
 
 class SingleStage:
     def __init__(self, block: SingleBlockLoRA):
@@ -66,6 +69,9 @@ class SingleStage:
     def apply_adamw(self, grads, lr: float) -> None:
         self.block.apply_adamw(grads, lr)
 
+    def apply_muon(self, grads, lr: float, **kw) -> None:
+        self.block.apply_muon(grads, lr, **kw)
+
 
 class JoinStage:
     """cat([txt, img]) along tokens (throughput.rs:545-550 order)."""
@@ -81,6 +87,9 @@ class JoinStage:
         return None, [g[:self.T].contiguous(), g[self.T:].contiguous()], {}
 
     def apply_adamw(self, grads, lr: float) -> None:
+        pass
+
+    def apply_muon(self, grads, lr: float, **kw) -> None:
         pass
 
 
@@ -140,3 +149,11 @@ def apply_adamw(stages: Sequence, grads: Dict[int, dict], lr: float = 1e-3) -> N
     for k, st in enumerate(stages):
         if grads.get(k):
             st.apply_adamw(grads[k], lr)
+
+
+def apply_muon(stages: Sequence, grads: Dict[int, dict], lr: float = 0.02, **kw) -> None:
+    """One orthogonalised step (block.muon_step_many, its options in kw) on
+    every stage's LoRA factors, in place of apply_adamw."""
+    for k, st in enumerate(stages):
+        if grads.get(k):
+            st.apply_muon(grads[k], lr, **kw)
