@@ -247,9 +247,15 @@ __device__ __forceinline__ void clamp_tokens(const Tile &t, int x, int (&token)[
 // ---------------------------------------------------------------------------
 // loads and operands
 // ---------------------------------------------------------------------------
-// 16 bytes from column c of a row of n elements; zero past its end.  FULL: they
-// all lie in the row (where a whole wave knows that, its loads need no branches).
-template <bool FULL = false, typename T>
+// A wave's last step over a row of W elements begins where it ends with the row,
+// so that all its loads lie in the row; `lo` is the first column that it has to
+// do (the ones before it are another step's).  Only rows shorter than a step
+// (FULL false) are loaded with a look at their end.
+__device__ __forceinline__ int64_t step_base(int64_t lo, int step, int64_t W) {
+    return W >= step ? std::min<int64_t>(lo, W - step) : lo;
+}
+// 16 bytes from column c of a row of n elements; past its end zero (FULL: none is)
+template <bool FULL, typename T>
 __device__ __forceinline__ u32x4 load16(const T *row, int64_t c, int64_t n) {
     constexpr int E = 16 / sizeof(T);
     if (FULL || c + E <= n) return *reinterpret_cast<const u32x4_any *>(row + c);
@@ -261,10 +267,11 @@ __device__ __forceinline__ u32x4 load16(const T *row, int64_t c, int64_t n) {
     __builtin_memcpy(&r, v, 16);
     return r;
 }
+// Columns lo .. n of 16 bytes at column c.
 template <typename T>
-__device__ __forceinline__ void store16(T *row, int64_t c, int64_t n, u32x4 w) {
+__device__ __forceinline__ void store16(T *row, int64_t c, int64_t lo, int64_t n, u32x4 w) {
     constexpr int E = 16 / sizeof(T);
-    if (c + E <= n) {
+    if (c >= lo && c + E <= n) {
         *reinterpret_cast<u32x4_any *>(row + c) = w;
         return;
     }
@@ -272,10 +279,40 @@ __device__ __forceinline__ void store16(T *row, int64_t c, int64_t n, u32x4 w) {
     __builtin_memcpy(v, &w, 16);
 #pragma unroll
     for (int j = 0; j < E; ++j)
-        if (c + j < n) row[c + j] = v[j];
+        if (c + j >= lo && c + j < n) row[c + j] = v[j];
+}
+// v with its first n elements zero
+template <typename T>
+__device__ __forceinline__ u32x4 zero_before(int n, u32x4 v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 2)
+            v[k] = n <= 2 * k ? v[k] : n == 2 * k + 1 ? v[k] & 0xffff0000u : 0u;
+        else
+            v[k] = n <= k ? v[k] : 0u;
+    }
+    return v;
 }
 __device__ __forceinline__ u32x4 zero_unless(bool keep, u32x4 v) {
     return u32x4{keep ? v[0] : 0u, keep ? v[1] : 0u, keep ? v[2] : 0u, keep ? v[3] : 0u};
+}
+// Ranks i .. of a row of r, zero past its end.  KIND 0: r fills its blocks of 16;
+// 1: a multiple of 4; 2: any, with branches.
+inline int rank_kind(int r) { return r % 16 == 0 ? 0 : r % 4 == 0 ? 1 : 2; }
+template <int KIND>
+__device__ __forceinline__ u32x4 load_ranks(const bf16 *row, int i, int r) {
+    if constexpr (KIND == 1) {
+        typedef u32x2 u32x2_any __attribute__((aligned(2)));
+        const u32x2 lo = *reinterpret_cast<const u32x2_any *>(row + std::min(i, r - 4));
+        const u32x2 hi = *reinterpret_cast<const u32x2_any *>(row + std::min(i + 4, r - 4));
+        return u32x4{i < r ? lo[0] : 0u, i < r ? lo[1] : 0u, i + 4 < r ? hi[0] : 0u, i + 4 < r ? hi[1] : 0u};
+    }
+    return load16<KIND == 0>(row, i, r);
+}
+template <int KIND>
+__device__ __forceinline__ u32x4 load_ranks(const float *row, int i, int r) {
+    if constexpr (KIND == 1) return zero_unless(i < r, *reinterpret_cast<const u32x4_any *>(row + std::min(i, r - 4)));
+    return load16<KIND == 0>(row, i, r);
 }
 __device__ __forceinline__ f32x4 load_f4(const float *base, int left) {
     if (left >= 4) return *reinterpret_cast<const f32x4_any *>(base);
@@ -364,9 +401,10 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
         for (int i = 0; i < 4; ++i) acc[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     u32x4 f[RB][2], d[4][2];
     // a factor row past the rank is the last one's again: its sums are not stored
-    auto load_step = [&](auto full, int64_t s) __attribute__((always_inline)) {
+    auto load_step = [&](auto full, int64_t lo) __attribute__((always_inline)) {
         constexpr bool FULL = decltype(full)::value;
-        const int64_t c = s * STEP + E * q;  // its loads h: columns c + 4 E h, 64 contiguous bytes a row
+        const int64_t base = step_base(lo, STEP, W);
+        const int64_t c = base + E * q;  // its loads h: columns c + 4 E h, 64 contiguous bytes a row
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
@@ -393,8 +431,8 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
         }
     };
     auto load = [&](int64_t s) __attribute__((always_inline)) {
-        if ((s + 1) * STEP <= W) load_step(std::true_type{}, s);
-        else load_step(std::false_type{}, s);
+        if (W >= STEP) load_step(std::true_type{}, s * STEP);
+        else load_step(std::false_type{}, s * STEP);
     };
     int64_t s = s0 + wave;
     if (s < s1) load(s);
@@ -407,8 +445,18 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) dc[i][h] = d[i][h];
         }
+        const int64_t lo = s * STEP, base = step_base(lo, STEP, W);
         s += 4;
         if (s < s1) load(s);
+        if (base < lo)  // both operands: a product of what is not this step's must not be NaN
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int n = (int)(lo - base) - E * q - 4 * E * h;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dc[i][h] = zero_before<T>(n, dc[i][h]);
+#pragma unroll
+                for (int b = 0; b < RB; ++b) fc[b][h] = zero_before<T>(n, fc[b][h]);
+            }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
@@ -449,7 +497,7 @@ constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
 constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
 
-template <typename T, int RB, bool ROWMAJOR>
+template <typename T, int RB, bool ROWMAJOR, int KIND>
 __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
     constexpr int PITCH = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
@@ -484,9 +532,9 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     u32x4 y[4][NY];
     u32x4 f[ROWMAJOR ? 4 : 1][RB];  // ROWMAJOR: the four products' operands
     u32x4 g[ROWMAJOR ? 1 : RB][ROWMAJOR ? 1 : 8 / E * 2];  // else rows as they lie, to be staged
-    const bool whole_rank = r == 16 * RB;
     auto load_step = [&](auto full, int64_t col) __attribute__((always_inline)) {
         constexpr bool FULL = decltype(full)::value;
+        col = step_base(col, kUpStep, W);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < subs) {
@@ -494,14 +542,15 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                 for (int n = 0; n < NY; ++n) y[i][n] = load16<FULL>(out[i], col + RUN * n + E * q, W);
             }
         if constexpr (ROWMAJOR) {
-            // a column past the row's end is the last one's again: its sums are not stored
+            // of a row shorter than the step, a column past its end is the last one's again: not stored
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const T *row = factor + std::min<int64_t>(col + column(j, x), W - 1) * r;
+                const int64_t c = col + column(j, x);
+                const T *row = factor + (FULL ? c : std::min<int64_t>(c, W - 1)) * r;
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const int k = sizeof(T) == 2 ? 16 * b + 8 * (q & 1) : 16 * b + 4 * q;
-                    f[j][b] = load16<FULL>(row, k, r);
+                    f[j][b] = load_ranks<KIND>(row, k, r);
                 }
             }
         } else {
@@ -517,7 +566,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
         }
     };
     auto load = [&](int64_t col) __attribute__((always_inline)) {
-        if (col + kUpStep <= W && (!ROWMAJOR || whole_rank)) load_step(std::true_type{}, col);
+        if (W >= kUpStep) load_step(std::true_type{}, col);
         else load_step(std::false_type{}, col);
     };
     if (live && c0 < W) load(c0);
@@ -530,7 +579,8 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
             for (int k = 0; k < p.splits; ++k)
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
-                    s[b] += load_f4(p.low + ((int64_t)k * p.T + ltoken) * r + 16 * b + 4 * h, r - 16 * b - 4 * h);
+                    s[b] += __builtin_bit_cast(
+                        f32x4, load_ranks<KIND>(p.low + ((int64_t)k * p.T + ltoken) * r, 16 * b + 4 * h, r));
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
             if (p.low_out && blockIdx.x == 0 && lrow < t.rows)  // the parts' sum, for the backward
@@ -603,7 +653,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
-        const int64_t c = c0 + E * q;
+        const int64_t lo = c0, c = step_base(c0, kUpStep, W) + E * q;
         c0 += step;
         if (c0 < W) load(c0);
 #pragma unroll
@@ -624,9 +674,9 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                     bf16x8 o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[e] = f32_to_bf16((float)old[e] + acc[2 * n + e / 4][e % 4]);
-                    store16(out[i], c + RUN * n, W, as_u32x4(o));
+                    store16(out[i], c + RUN * n, lo, W, as_u32x4(o));
                 } else {
-                    store16(out[i], c + RUN * n, W,
+                    store16(out[i], c + RUN * n, lo, W,
                             __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, yc[i][n]) + acc[n]));
                 }
             }
@@ -665,7 +715,7 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const int pair = wave >> 1;
     const int r = p.r, W = p.wide;
-    const int64_t base = ((int64_t)block * 2 + (wave & 1)) * 16 * E, c = base + E * x;
+    const int64_t lo = ((int64_t)block * 2 + (wave & 1)) * 16 * E, c = step_base(lo, 16 * E, W) + E * x;
     const int steps = (t.rows + kGradRows - 1) / kGradRows;
     {
         // rows past the end: the first one's token, negative (~token)
@@ -686,25 +736,26 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
         }
     };
     auto load_wide = [&](int s) __attribute__((always_inline)) {
-        if (base + 16 * E <= W) load_rows(std::true_type{}, s);
+        if (W >= 16 * E) load_rows(std::true_type{}, s);
         else load_rows(std::false_type{}, s);
     };
-    const bool any = base < W;
+    const bool any = lo < W;
     if (any && pair < steps) load_wide(pair);
     if constexpr (sizeof(T) == 2) {
         // thread: rank i % 16, rows 8 (i / 16) .. + 8
-        for (int i = threadIdx.x; i < 2 * kChunk && i / 16 * 8 < steps * kGradRows; i += 256) {
+#pragma unroll
+        for (int n = 0; n < 2 * kChunk / 256; ++n) {
+            const int i = n * 256 + threadIdx.x;
             const int rank = i % 16, row = i / 16 * 8;
             float low[RB][8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int token = lds.token[row + e];
+                const float *src = p.low + (int64_t)(token < 0 ? ~token : token) * r;
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
-                    float w = 0.f;
-                    if (token >= 0 && 16 * b + rank < r)
-                        for (int k = 0; k < p.splits; ++k) w += p.low[((int64_t)k * p.T + token) * r + 16 * b + rank];
-                    low[b][e] = w;
+                    const float w = src[std::min(16 * b + rank, r - 1)];
+                    low[b][e] = token >= 0 && 16 * b + rank < r ? w : 0.f;
                 }
             }
 #pragma unroll
@@ -716,12 +767,11 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
             }
         }
     } else {
-        for (int i = threadIdx.x; i < kChunk * RB * 16; i += 256) {
-            const int row = i / (RB * 16), rank = i % (RB * 16), token = lds.token[row];
-            float w = 0.f;
-            if (token >= 0 && rank < r)
-                for (int k = 0; k < p.splits; ++k) w += p.low[((int64_t)k * p.T + token) * r + rank];
-            lds.low[row][rank] = w;
+#pragma unroll 16
+        for (int n = 0; n < RB * 16; ++n) {
+            const int i = n * 256 + threadIdx.x, row = i / (RB * 16), rank = i % (RB * 16), token = lds.token[row];
+            const float w = p.low[(int64_t)(token < 0 ? ~token : token) * r + std::min(rank, r - 1)];
+            lds.low[row][rank] = token >= 0 && rank < r ? w : 0.f;
         }
     }
     __syncthreads();
@@ -788,7 +838,7 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
         if (g.transpose) {  // [wide][r]
 #pragma unroll
             for (int j = 0; j < E; ++j)
-                if (c + j < W) store_f4(out + (c + j) * r + i, r - i, acc[b][j] * scale);
+                if (c + j >= lo && c + j < W) store_f4(out + (c + j) * r + i, r - i, acc[b][j] * scale);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -796,8 +846,9 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
                 float *row = out + (int64_t)(i + e) * W;
 #pragma unroll
                 for (int j = 0; j < E; j += 4)
-                    store_f4(row + c + j, (int)std::min<int64_t>(4, W - c - j),
-                             f32x4{acc[b][j][e], acc[b][j + 1][e], acc[b][j + 2][e], acc[b][j + 3][e]} * scale);
+                    store16(row, c + j, lo, W,
+                            __builtin_bit_cast(u32x4, f32x4{acc[b][j][e], acc[b][j + 1][e], acc[b][j + 2][e],
+                                                            acc[b][j + 3][e]} * scale));
             }
         }
     }
@@ -880,19 +931,27 @@ hipError_t down_t(const PoolParams &p, hipStream_t s) {
     }
     return hipGetLastError();
 }
-template <typename T, bool ROWMAJOR>
-hipError_t up_t(const PoolParams &p, hipStream_t s) {
+template <typename T, bool ROWMAJOR, int KIND>
+hipError_t up_kind(const PoolParams &p, hipStream_t s) {
     // two steps a wave where one each would not all fit the chip at once (three workgroups a CU)
     const int64_t tiles = most_tiles(p.T, p.L, kRows), blocks = ((int64_t)p.wide + 4 * kUpStep - 1) / (4 * kUpStep);
     const int64_t turns = tiles * blocks > 3 * (int64_t)device_cu_count() ? 2 : 1;
     const dim3 grid = tile_grid((blocks + turns - 1) / turns, tiles), block(256);
     switch ((p.r + 15) / 16) {
-        case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
-        case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
-        case 3: hipLaunchKernelGGL((pool_up_kernel<T, 3, ROWMAJOR>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((pool_up_kernel<T, 4, ROWMAJOR>), grid, block, 0, s, p); break;
+        case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
+        case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
+        case 3: hipLaunchKernelGGL((pool_up_kernel<T, 3, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((pool_up_kernel<T, 4, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
     }
     return hipGetLastError();
+}
+template <typename T, bool ROWMAJOR>
+hipError_t up_t(const PoolParams &p, hipStream_t s) {
+    switch (rank_kind(p.r)) {
+        case 0: return up_kind<T, ROWMAJOR, 0>(p, s);
+        case 1: return up_kind<T, ROWMAJOR, 1>(p, s);
+        default: return up_kind<T, ROWMAJOR, 2>(p, s);
+    }
 }
 template <typename T>
 hipError_t grad_t(const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb, const PoolGradParams &gb,

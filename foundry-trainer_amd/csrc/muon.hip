@@ -51,8 +51,12 @@ struct Place {
     int slot;        // over all items
 };
 __device__ __forceinline__ Place place_of(const MuonMany &p, int b) {
-    int k = 0;
-    while (k + 1 < p.items && p.block0[k + 1] <= b) ++k;
+    int k = 0, end = p.items - 1;  // the last item that begins at or before b
+    while (k < end) {
+        const int mid = (k + end + 1) / 2;
+        if (p.block0[mid] <= b) k = mid;
+        else end = mid - 1;
+    }
     const int local = b - p.block0[k];
     Place w;
     w.item = k;
@@ -154,8 +158,12 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
     extern __shared__ double lds[];  // G, Q, T and H = G Q, each [RB][RB] tiles of [4][64]
     double *G = lds, *Q = lds + ALL, *T = lds + 2 * ALL, *H = lds + 3 * ALL;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int k = 0;
-    while (k + 1 < p.items && p.matrix0[k + 1] <= (int)blockIdx.x) ++k;
+    int k = 0, end = p.items - 1;
+    while (k < end) {
+        const int mid = (k + end + 1) / 2;
+        if (p.matrix0[mid] <= (int)blockIdx.x) k = mid;
+        else end = mid - 1;
+    }
     const int64_t matrix = blockIdx.x - p.matrix0[k];
     const int chunks = p.chunks[k];
     const double *part = p.gram + (p.gram0[k] + matrix * chunks * (int64_t)(NT * kTile));
