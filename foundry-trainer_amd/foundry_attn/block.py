@@ -36,6 +36,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass, field
 from typing import Dict, Optional, Sequence, Tuple
@@ -157,6 +158,12 @@ def layer_norm_fwd(x, weight, bias=None, eps: float = 1e-5, out=None):
     return y, mean, rstd
 
 
+@functools.lru_cache(maxsize=4096)
+def _layer_norm_bytes(device: int, *sizes) -> int:
+    """Workspace bytes of layer_norm_bwd for dtypes and sizes on `device`."""
+    return max(_abi.entry("fa_layer_norm_bwd_workspace_size", size=True)(_pack_layer_norm_bwd(*sizes, *(0,) * 19)), 256)
+
+
 def layer_norm_bwd(x, dy, weight, mean, rstd, dres=None, out=None, want_dweight: bool = True,
                    want_dbias: bool = True):
     """(dx, dweight, dbias) of layer_norm_fwd for the upstream gradient dy,
@@ -180,7 +187,7 @@ def layer_norm_bwd(x, dy, weight, mean, rstd, dres=None, out=None, want_dweight:
             0 if dres is None else dres.stride(0), dx.data_ptr(), dx.stride(0), _ptr(dw), _ptr(db))
     ws, size = None, 0
     if want_dweight or want_dbias:
-        size = max(_abi.entry("fa_layer_norm_bwd_workspace_size", size=True)(_pack_layer_norm_bwd(*head, 0, 0)), 256)
+        size = _layer_norm_bytes(x.get_device(), *head[:4])
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
     _abi.call("fa_layer_norm_bwd", _pack_layer_norm_bwd(*head, _ptr(ws), size), stream)
     return dx, dw, db

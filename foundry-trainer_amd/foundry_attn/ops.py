@@ -20,6 +20,7 @@ device memory and streams here; all arithmetic is in the HIP kernels.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import weakref
 from typing import Optional, Sequence, Tuple
@@ -642,8 +643,17 @@ class LoraPoolPlan:
 def _plan_call(index, plan: LoraPoolPlan) -> None:
     if index.dtype != torch.int32 or not index.is_contiguous():
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "index must be contiguous int32")
-    check(lib().fa_lora_pool_plan(index.data_ptr(), plan.tokens, plan.adapters, plan.data.data_ptr(),
-                                  plan.data.numel(), _stream(index)))
+    status = lib().fa_lora_pool_plan(index.data_ptr(), plan.tokens, plan.adapters, plan.data.data_ptr(),
+                                     plan.data.numel(), _stream(index))
+    if status != _abi.FA_OK:
+        check(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(tokens: int, adapters: int) -> int:
+    if not 1 <= adapters <= 2048 or tokens > 1 << 28:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{adapters} adapters, {tokens} tokens: 1..2048 and up to 2^28")
+    return lib().fa_lora_pool_plan_size(tokens, adapters)
 
 
 def lora_pool_plan(index, adapters: int) -> LoraPoolPlan:
@@ -654,18 +664,16 @@ def lora_pool_plan(index, adapters: int) -> LoraPoolPlan:
     if index.dim() != 1 or not index.is_cuda:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "index must be a 1-D device tensor")
     tokens, adapters = index.shape[0], int(adapters)
-    if not 1 <= adapters <= 2048 or tokens > 1 << 28:
-        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{adapters} adapters, {tokens} tokens: 1..2048 and up to 2^28")
-    size = lib().fa_lora_pool_plan_size(tokens, adapters)
-    plan = LoraPoolPlan(tokens, adapters, torch.empty(size, dtype=torch.uint8, device=index.device))
+    data = torch.empty(_plan_bytes(tokens, adapters), dtype=torch.uint8, device=index.device)
+    plan = LoraPoolPlan(tokens, adapters, data)
     _plan_call(index, plan)
     return plan
 
 
-def _pool_rows(t, tokens: int, n: int, like, name: str):
-    if t.shape != (tokens, n) or (n > 1 and t.stride(1) != 1) or t.dtype != like.dtype or t.device != like.device:
+def _pool_rows(t, shape: tuple, like, name: str):
+    if t.shape != shape or (shape[1] > 1 and t.stride(1) != 1) or t.dtype != like.dtype or t.device != like.device:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
-                               f"{name} must be {like.dtype} [{tokens}, {n}] with contiguous rows on {like.device}")
+                               f"{name} must be {like.dtype} {list(shape)} with contiguous rows on {like.device}")
     return t
 
 
@@ -674,14 +682,13 @@ def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u) -> tuple:
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or not x.is_cuda:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "x must be [T, K] on the device, a [L, r, K], b [L, M, r]")
     T, K = x.shape
-    L, r = a.shape[:2]
-    M = b.shape[1]
-    if a.shape != (L, r, K) or b.shape != (L, M, r):
+    L, r, ka = a.shape
+    lb, M, rb = b.shape
+    if (lb, rb, ka) != (L, r, K):
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "a must be [L, r, K], b [L, M, r]")
     dev, dt = x.device, x.dtype
-    for name, t in (("a", a), ("b", b)):
-        if t.dtype != dt or t.device != dev or not t.is_contiguous():
-            raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"{name} must be contiguous {dt} on {dev}")
+    if not (a.dtype == b.dtype == dt and a.device == b.device == dev and a.is_contiguous() and b.is_contiguous()):
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"a and b must be contiguous {dt} on {dev}")
     if scales.shape != (L,) or scales.dtype != torch.float32 or not scales.is_contiguous() or scales.device != dev:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"scales must be contiguous float32 [{L}] on {dev}")
     if plan.tokens != T or plan.adapters != L or plan.data.device != dev:
@@ -689,9 +696,19 @@ def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u) -> tuple:
                                                         f"adapters, the call of {T} and {L}")
     if u.shape != (T, r) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"u must be contiguous float32 [{T}, {r}] on {dev}")
-    _pool_rows(x, T, K, x, "x")
+    if K > 1 and x.stride(1) != 1:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "x must have contiguous rows")
     return (_dtype_code(x), T, K, M, r, L, x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
             plan.data.data_ptr(), plan.data.numel(), u.data_ptr())
+
+
+@functools.lru_cache(maxsize=4096)
+def _pool_bytes(device: int, backward: bool, *sizes) -> int:
+    """Workspace bytes of a call with these dtype, T, K, M, r and L on `device`."""
+    if backward:
+        pack = _pack_pool_bwd(*sizes, *(0,) * 18)
+        return max(_abi.entry("fa_lora_pool_bwd_workspace_size", size=True)(pack), 256)
+    return _abi.entry("fa_lora_pool_fwd_workspace_size", size=True)(_pack_pool(*sizes, *(0,) * 12))
 
 
 def lora_pool_fwd(x, a, b, y, scales, plan: LoraPoolPlan):
@@ -701,12 +718,11 @@ def lora_pool_fwd(x, a, b, y, scales, plan: LoraPoolPlan):
     [T, r], zero rows without an adapter) for the backward."""
     u = torch.empty((x.shape[0], a.shape[1]), dtype=torch.float32, device=x.device)
     head = _pool_args(x, a, b, scales, plan, u)
-    _pool_rows(y, x.shape[0], b.shape[1], x, "y")
-    head += (y.data_ptr(), y.stride(0))
+    _pool_rows(y, (head[1], head[3]), x, "y")
     stream = _stream(x)
-    need = _abi.entry("fa_lora_pool_fwd_workspace_size", size=True)(_pack_pool(*head, 0, 0))
+    need = _pool_bytes(x.get_device(), False, *head[:6])
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _abi.call("fa_lora_pool_fwd", _pack_pool(*head, _ptr(ws), need), stream)
+    _abi.call("fa_lora_pool_fwd", _pack_pool(*head, y.data_ptr(), y.stride(0), _ptr(ws), need), stream)
     return u
 
 
@@ -715,17 +731,16 @@ def lora_pool_bwd(x, a, b, u, dy, scales, plan: LoraPoolPlan, dx=None, want_fact
     gradient dy (zero for adapters without tokens; None each without
     want_factors); dx[t] += scales[i] A_i^T (B_i^T dy[t]) when given."""
     head = _pool_args(x, a, b, scales, plan, u)
-    _pool_rows(dy, x.shape[0], b.shape[1], x, "dy")
+    _pool_rows(dy, (head[1], head[3]), x, "dy")
     if dx is not None:
-        _pool_rows(dx, x.shape[0], x.shape[1], x, "dx")
+        _pool_rows(dx, (head[1], head[2]), x, "dx")
     stream = _stream(x)
     da = db = None
     if want_factors:
         da = torch.empty(a.shape, dtype=torch.float32, device=x.device)
         db = torch.empty(b.shape, dtype=torch.float32, device=x.device)
     tail = (dy.data_ptr(), dy.stride(0), _ptr(da), _ptr(db), _ptr(dx), 0 if dx is None else dx.stride(0))
-    size = _abi.entry("fa_lora_pool_bwd_workspace_size", size=True)
-    need = max(size(_pack_pool_bwd(*head, 0, 0, 0, 0, *tail)), 256)
+    need = _pool_bytes(x.get_device(), True, *head[:6])
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _abi.call("fa_lora_pool_bwd", _pack_pool_bwd(*head, 0, 0, ws.data_ptr(), need, *tail), stream)
     return da, db
