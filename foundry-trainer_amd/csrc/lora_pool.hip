@@ -122,13 +122,17 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
         }
         return same;
     };
+    const uint64_t below = (uint64_t(1) << lane) - 1;
     int ahead = adapter_of(t0 + lane);
 #pragma unroll 1
     for (int64_t t = t0; t < t1; t += 64) {
         const int a = ahead;
         ahead = adapter_of(t + 64 + lane);
         const uint64_t same = peers(a);
-        if (a >= 0 && lane == __builtin_ctzll(same)) hist[wave * A + a] += __popcll(same);
+        if (a < 0) continue;
+        const int n = hist[wave * A + a];
+        if (kept) idx[t + lane] = (n + __popcll(same & below)) << 12 | a;  // its place among the wave's of its adapter
+        if (lane == __builtin_ctzll(same)) hist[wave * A + a] = n + __popcll(same);
     }
     __syncthreads();
     if (wave == 0) {
@@ -168,20 +172,24 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
             total[1] = chunks0[A] = chunks;
             *reinterpret_cast<u32x4 *>(v.head) = u32x4{(uint32_t)tiles, (uint32_t)chunks, (uint32_t)T, (uint32_t)L};
         }
-    } else {
-        ahead = adapter_of(t0 + lane);
     }
     __syncthreads();
-    if (wave == 0) ahead = adapter_of(t0 + lane);
+    if (kept) {
+        for (int64_t t = t0 + lane; t < t1; t += 64) {
+            const int w = idx[t];
+            v.token[hist[wave * A + (w & 4095)] + (w >> 12)] = (int)t;
+        }
+    } else {
+        ahead = adapter_of(t0 + lane);
 #pragma unroll 1
-    for (int64_t t = t0; t < t1; t += 64) {
-        const int a = ahead;
-        ahead = adapter_of(t + 64 + lane);
-        const uint64_t same = peers(a);
-        if (a >= 0) {
-            const int at = hist[wave * A + a];
-            v.token[at + __popcll(same & ((uint64_t(1) << lane) - 1))] = (int)t + lane;
-            if (lane == __builtin_ctzll(same)) hist[wave * A + a] = at + __popcll(same);
+        for (int64_t t = t0; t < t1; t += 64) {
+            const int a = ahead;
+            ahead = adapter_of(t + 64 + lane);
+            const uint64_t same = peers(a);
+            if (a < 0) continue;
+            const int n = hist[wave * A + a];
+            v.token[n + __popcll(same & below)] = (int)t + lane;
+            if (lane == __builtin_ctzll(same)) hist[wave * A + a] = n + __popcll(same);
         }
     }
     auto find = [&](const int *first, int i) {  // the last adapter a with first[a] <= i

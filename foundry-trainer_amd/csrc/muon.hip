@@ -26,6 +26,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fa_device.hpp"
 #include "fa_kernels.hpp"
@@ -76,6 +77,10 @@ __device__ __forceinline__ f32x4 load4(const float *base, int64_t at, int64_t st
         if (e < left) v[e] = base[at + e * step];
     return v;
 }
+__device__ __forceinline__ f32x4 load_full(const float *base, int64_t at, int64_t step) {
+    if (step == 1) return *reinterpret_cast<const f32x4_any *>(base + at);
+    return f32x4{base[at], base[at + step], base[at + 2 * step], base[at + 3 * step]};
+}
 __device__ __forceinline__ void store4(float *base, int64_t at, int64_t step, int left, f32x4 v) {
     if (step == 1 && left >= 4) {
         *reinterpret_cast<f32x4_any *>(base + at) = v;
@@ -92,7 +97,7 @@ __device__ __forceinline__ void store4(float *base, int64_t at, int64_t step, in
 template <int RB>
 __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
     constexpr int NT = RB * (RB + 1) / 2;
-    __shared__ double sum[NT * kTile];
+    __shared__ double sum[4][NT * kTile];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Place at = place_of(p, blockIdx.x);
     const int k = at.item, r = p.r[k], n = p.n[k];
@@ -106,43 +111,58 @@ __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
     f64x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f64x4{0, 0, 0, 0};
-    for (int j = j0 + wave * 16; j < j1; j += 64) {
-        const int jl = j + 4 * (lane >> 4);
-        f32x4 u[RB];
+    // AT_ONCE steps at once: their loads go out side by side.  FULL: all of the
+    // steps' columns and rows are there, and the loads need no branches.
+    auto do_steps = [&](auto full, auto at_once, int j) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
+        constexpr int STEPS = decltype(at_once)::value;
+        f32x4 gv[STEPS][RB], mv[STEPS][RB];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            const int i = 16 * b + (lane & 15);
-            const int left = i < r ? j1 - jl : 0;
-            const int64_t e = i * rs + jl * cs;
-            const f32x4 gv = load4(g, e, cs, left), mv = load4(m, e, cs, left);
-            f32x4 mn;
+        for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                mn[q] = __builtin_fmaf(beta, mv[q], gv[q]);
-                u[b][q] = p.nesterov ? __builtin_fmaf(beta, mn[q], gv[q]) : mn[q];
+            for (int b = 0; b < RB; ++b) {
+                const int i = 16 * b + (lane & 15), jl = j + 64 * s + 4 * (lane >> 4);
+                const int64_t e = i * rs + jl * cs;
+                const int left = i < r ? j1 - jl : 0;
+                gv[s][b] = FULL ? load_full(g, e, cs) : load4(g, e, cs, left);
+                mv[s][b] = FULL ? load_full(m, e, cs) : load4(m, e, cs, left);
             }
-            store4(m, e, cs, left, mn);
-        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int s = 0; s < STEPS; ++s) {
+            f32x4 u[RB];
 #pragma unroll
-            for (int b = 0, t = 0; b < RB; ++b)
+            for (int b = 0; b < RB; ++b) {
+                const int i = 16 * b + (lane & 15), jl = j + 64 * s + 4 * (lane >> 4);
+                f32x4 mn;
 #pragma unroll
-                for (int c = b; c < RB; ++c, ++t) acc[t] = mfma_f64((double)u[b][q], (double)u[c][q], acc[t]);
-    }
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    double *s = &sum[t * kTile + i * 64 + lane];
-                    *s = w ? *s + acc[t][i] : acc[t][i];
+                for (int q = 0; q < 4; ++q) {
+                    mn[q] = __builtin_fmaf(beta, mv[s][b][q], gv[s][b][q]);
+                    u[b][q] = p.nesterov ? __builtin_fmaf(beta, mn[q], gv[s][b][q]) : mn[q];
                 }
-        __syncthreads();
-    }
+                store4(m, i * rs + jl * cs, cs, FULL ? 4 : i < r ? j1 - jl : 0, mn);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int b = 0, t = 0; b < RB; ++b)
+#pragma unroll
+                    for (int c = b; c < RB; ++c, ++t) acc[t] = mfma_f64((double)u[b][q], (double)u[c][q], acc[t]);
+        }
+    };
+    constexpr int AT_ONCE = RB <= 2 ? 2 : 1;
+    int j = j0 + wave * 16;
+    if (r == 16 * RB)
+        for (; j + 64 * (AT_ONCE - 1) + 16 <= j1; j += 64 * AT_ONCE)
+            do_steps(std::true_type{}, std::integral_constant<int, AT_ONCE>{}, j);
+    for (; j < j1; j += 64) do_steps(std::false_type{}, std::integral_constant<int, 1>{}, j);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[wave][t * kTile + i * 64 + lane] = acc[t][i];
+    __syncthreads();
     double *out = p.gram + (p.gram0[k] + (at.matrix * p.chunks[k] + at.chunk) * (int64_t)(NT * kTile));
-    for (int i = threadIdx.x; i < NT * kTile; i += 256) out[i] = sum[i];
+#pragma unroll
+    for (int i = threadIdx.x; i < NT * kTile; i += 256) out[i] = sum[0][i] + sum[1][i] + sum[2][i] + sum[3][i];
 }
 
 // T of one matrix.  Element i of a tile in lane l is (row 4 i + l / 16, column
