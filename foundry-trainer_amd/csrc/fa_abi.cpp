@@ -1384,8 +1384,9 @@ fa_status check_muon(const fa_muon_args *a) {
         !aligned(a->momentum, 4))
         return fail(FA_ERR_INVALID_ARG, "param/grad/momentum is NULL or misaligned");
     if (!(a->lr >= 0.0) || !isfinite(a->lr) || !(a->beta >= 0.0 && a->beta < 1.0) || !(a->weight_decay >= 0.0) ||
-        !(a->lr * a->weight_decay <= 1.0) || !(a->eps > 0.0) || !isfinite(a->eps))
-        return fail(FA_ERR_INVALID_ARG, "need finite lr >= 0, 0 <= beta < 1, 0 <= lr * weight_decay <= 1, finite eps > 0");
+        !(a->lr * a->weight_decay <= 1.0) || !(a->eps >= 1e-300) || !isfinite(a->eps))
+        return fail(FA_ERR_INVALID_ARG,
+                    "need finite lr >= 0, 0 <= beta < 1, 0 <= lr * weight_decay <= 1, finite eps >= 1e-300");
     if (!isfinite(a->scale) || !isfinite(a->a) || !isfinite(a->b) || !isfinite(a->c))
         return fail(FA_ERR_INVALID_ARG, "scale and the coefficients must be finite");
     if (a->steps < 0 || a->steps > FA_MUON_MAX_STEPS)

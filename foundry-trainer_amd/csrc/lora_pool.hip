@@ -231,7 +231,7 @@ __device__ __forceinline__ bool tile_of(const PoolParams &p, const PlanView &v, 
     t = __builtin_bit_cast(Tile, w);
     const int n = (int)(chunk ? head[1] : head[0]), most = chunk ? kChunk : kRows;
     return (int)head[2] == p.T && (int)head[3] == p.L && i < n && t.tile >= 0 && t.rows > 0 && t.rows <= most &&
-           t.tile + (t.rows + kRows - 1) / kRows <= most_tiles(p.T, p.L, kRows) && t.adapter < p.L;
+           (int64_t)t.tile + (t.rows + kRows - 1) / kRows <= most_tiles(p.T, p.L, kRows) && t.adapter < p.L;
 }
 // The token in entry `at` of the plan's list; 0 where it holds no token.
 __device__ __forceinline__ int token_at(const PoolParams &p, const PlanView &v, int64_t at) {
@@ -363,7 +363,7 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TE
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             t[j] = f32_to_bf16(rest[j]);
-            rest[j] -= (float)t[j];
+            rest[j] = __builtin_isfinite((float)t[j]) ? rest[j] - (float)t[j] : 0.f;
         }
         out[k] = as_u32x4(t);
     }
@@ -922,8 +922,9 @@ int down_splits(int T, int L, int W) {
     while (2 * splits <= std::min<int64_t>(std::min<int64_t>(want, 64), W / 256)) splits *= 2;
     return (int)splits;
 }
-// Partial gradients: chunks of adapters with more than one, at most two for each full one
-int64_t grad_slots(int T) { return 2 * ((int64_t)T / kChunk); }
+// Partial gradients: the chunks of adapters with more than one, all full but each
+// adapter's last
+int64_t grad_slots(int T, int L) { return (int64_t)T / kChunk + std::min<int64_t>(L, (int64_t)T / (kChunk + 1)); }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 size_t low_bytes(int T, int r, int splits) { return align256((size_t)splits * T * r * sizeof(float)); }
@@ -998,7 +999,7 @@ size_t pool_fwd_workspace_bytes(const PoolCall &c) {
 size_t pool_bwd_workspace_bytes(const PoolCall &c) {
     const int splits = down_splits(c.T, c.L, c.M);
     return low_bytes(c.T, c.r, splits) + (splits > 1 ? low_bytes(c.T, c.r, 1) : 0) +
-           align256((size_t)grad_slots(c.T) * c.r * ((size_t)c.K + c.M) * sizeof(float));
+           align256((size_t)grad_slots(c.T, c.L) * c.r * ((size_t)c.K + c.M) * sizeof(float));
 }
 
 static PoolParams pool_params(const PoolCall &c) {
@@ -1045,7 +1046,7 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
     const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
     const int cols = bf ? 256 : 128;
     ga.out = c.da;
-    ga.slots = gb.slots = (int)grad_slots(c.T);
+    ga.slots = gb.slots = (int)grad_slots(c.T, c.L);
     ga.part = part;
     ga.blocks = (c.K + cols - 1) / cols;
     gb.out = c.db;

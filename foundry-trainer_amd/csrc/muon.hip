@@ -161,7 +161,6 @@ __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
         for (int i = 0; i < 4; ++i) sum[wave][t * kTile + i * 64 + lane] = acc[t][i];
     __syncthreads();
     double *out = p.gram + (p.gram0[k] + (at.matrix * p.chunks[k] + at.chunk) * (int64_t)(NT * kTile));
-#pragma unroll
     for (int i = threadIdx.x; i < NT * kTile; i += 256) out[i] = sum[0][i] + sum[1][i] + sum[2][i] + sum[3][i];
 }
 
@@ -217,7 +216,7 @@ __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
     for (int u = 0; u < OWN; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            g[u][i] = mine ? tile(G, b0 + u, c0)[i * 64 + lane] * (inv * inv) : 0.0;
+            g[u][i] = mine ? tile(G, b0 + u, c0)[i * 64 + lane] * inv * inv : 0.0;  // inv * inv may be infinite
             t[u][i] = diagonal(u, i) ? 1.0 : 0.0;
         }
     const f64x4 zero = {0, 0, 0, 0};

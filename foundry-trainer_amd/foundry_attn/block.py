@@ -203,6 +203,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y.view(x.shape)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, weight, mean, rstd = ctx.saved_tensors
         wb = ctx.bias_dtype is not None and ctx.needs_input_grad[2]
@@ -406,7 +407,7 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
     if not first.is_cuda:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "params must be device tensors")
     ca, cb, cc = (float(v) for v in coeffs)
-    packed, count = [], 0
+    packed, count, seen = [], 0, set()
     for p, g, m in items:
         if p.dim() not in (2, 3) or not p.is_contiguous() or p.dtype != first.dtype or p.device != dev:
             raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
@@ -417,6 +418,7 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
                                        f"{name} must be contiguous float32 {list(p.shape)} on {dev}")
         if p.dim() == 3 and p.shape[0] == 0:
             continue
+        seen |= {p.data_ptr(), m.data_ptr()}
         rows, cols = p.shape[-2:]
         sc = math.sqrt(max(1.0, rows / max(cols, 1))) if scale is None else float(scale)
         packed.append(_pack_muon(code, p.shape[0] if p.dim() == 3 else 1, rows, cols, p.data_ptr(), g.data_ptr(),
@@ -425,6 +427,8 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
         count += 1
     if not count:
         return
+    if len(seen) != 2 * count:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "a param or momentum is listed twice")
     arr, stream = b"".join(packed), _stream(first)
     need = max(_abi.entry("fa_muon_step_many_workspace_size", ctypes.c_int32, size=True)(arr, count), 256)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)

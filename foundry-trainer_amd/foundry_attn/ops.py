@@ -754,10 +754,11 @@ class _LoraPoolFn(torch.autograd.Function):
         a, b = a.contiguous(), b.contiguous()
         u = lora_pool_fwd(x2, a, b, y.view(-1, y.shape[-1]), scales, plan)
         ctx.save_for_backward(x2, a, b, u, scales, plan.data)
-        ctx.plan = (plan.tokens, plan.adapters)
+        ctx.plan, ctx.x_shape = (plan.tokens, plan.adapters), x.shape
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, a, b, u, scales, data = ctx.saved_tensors
         dy2 = dy.reshape(-1, dy.shape[-1]).contiguous()
@@ -765,7 +766,7 @@ class _LoraPoolFn(torch.autograd.Function):
         da, db = lora_pool_bwd(x2, a, b, u, dy2, scales, LoraPoolPlan(*ctx.plan, data), dx=dx,
                                want_factors=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         cast = lambda g, t: None if g is None else g.to(t.dtype)
-        return (None if dx is None else dx.view(*dy.shape[:-1], -1), cast(da, a), cast(db, b), dy, None, None)
+        return (None if dx is None else dx.view(ctx.x_shape), cast(da, a), cast(db, b), dy, None, None)
 
 
 def lora_pool(x, a, b, base, scales, plan: LoraPoolPlan):

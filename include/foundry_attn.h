@@ -465,7 +465,8 @@ typedef struct fa_lora_pool_args {
 
 /* y[t] += scale_i B_i (A_i x[t]); rows of tokens without an adapter stay as
  * they are.  Any sizes and strides: rows and factors need their element's
- * alignment only.  Deterministic.  A plan of other tokens or adapters, or
+ * alignment only.  No output may overlap an input or another output (y may
+ * overlap x, which is read first).  Deterministic.  A plan of other tokens or adapters, or
  * memory that is no plan, gives wrong results but leads to no access outside
  * the call's tensors. */
 size_t fa_lora_pool_fwd_workspace_size(const fa_lora_pool_args *args);

@@ -258,7 +258,7 @@ typedef struct fa_muon_args {
     double lr;            /* >= 0                                                */
     double beta;          /* momentum, 0 <= beta < 1                             */
     double weight_decay;  /* decoupled, >= 0, lr * weight_decay <= 1             */
-    double eps;           /* > 0, added to the Frobenius norm                    */
+    double eps;           /* >= 1e-300, added to the Frobenius norm              */
     double scale;         /* of the orthogonalised update, e.g.
                              sqrt(max(1, rows / cols)); finite                   */
     double a, b, c;       /* coefficients of one product, finite                 */

@@ -269,3 +269,59 @@ def test_stream_and_graph(device):
         torch.cuda.synchronize()
         eager = run(d)
         assert all(torch.equal(outs[n], eager[n]) for n in eager), k
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_infinities_come_through(device, dt):
+    """An infinite activation of one token, rank 1: infinite where the formula
+    says so, NaN nowhere else, and the other tokens as they were."""
+    d = make(40, 2, 30, 24, 1, dt, seed=37)
+    t = (d["index"] == 1).nonzero().flatten()[0]
+    d["a"][1].abs_().add_(0.125)
+    d["b"][1].abs_().add_(0.125)
+    clean = run(d)
+    d["x"] = d["x"].clone()
+    d["x"][t] = d["x"][t].abs()
+    d["x"][t, 7] = float("inf")
+    got = run(d)
+    assert (got["u"][t] == float("inf")).all() and (got["y"][t] == float("inf")).all()
+    rest = torch.arange(40, device="cuda") != t
+    for k in ("u", "y", "dx"):
+        assert torch.equal(got[k][rest], clean[k][rest]), k
+    assert torch.equal(got["da"][0], clean["da"][0]) and torch.equal(got["db"][0], clean["db"][0])
+
+
+def test_wrappers_without_tokens(device):
+    d = make(0, 2, 16, 8, 4, F32)
+    leaves = {k: d[k].requires_grad_() for k in ("x", "a", "b")}
+    out = fa.lora_pool(leaves["x"].view(0, 1, 16), leaves["a"], leaves["b"], d["y"].view(0, 1, 8), d["scales"],
+                       fa.lora_pool_plan(d["index"], 2))
+    out.sum().backward()
+    assert leaves["x"].grad.shape == (0, 16) and not leaves["a"].grad.any() and not leaves["b"].grad.any()
+
+
+def test_y_over_x(device):
+    """y may be x itself where the widths agree: x is read first."""
+    d = make(100, 3, 48, 48, 8, BF, seed=41)
+    want = dict(d, y=d["x"].clone())
+    plan = fa.lora_pool_plan(d["index"], 3)
+    u0 = fa.lora_pool_fwd(d["x"], d["a"], d["b"], want["y"], d["scales"], plan)
+    x = d["x"].clone()
+    u1 = fa.lora_pool_fwd(x, d["a"], d["b"], x, d["scales"], plan)
+    assert torch.equal(x, want["y"]) and torch.equal(u0, u1)
+
+
+def test_memory_that_is_no_plan(device):
+    """Whatever lies in the plan's memory, nothing outside the call's tensors is
+    touched (the checks on every word of it are the host's arithmetic: indices
+    are compared as unsigned against the sizes before any use)."""
+    d = make(70, 3, 40, 24, 4, F32, seed=43)
+    plan = fa.lora_pool_plan(d["index"], 3)
+    words = plan.data.view(torch.int32)
+    other = fa.lora_pool_plan(torch.zeros(69, dtype=torch.int32, device="cuda"), 3)
+    words.zero_()  # sizes that are not the call's: nothing is done
+    y = d["y"].clone()
+    fa.lora_pool_fwd(d["x"], d["a"], d["b"], y, d["scales"], plan)
+    assert torch.equal(y, d["y"])
+    with pytest.raises(fa.FoundryAttnError):
+        fa.lora_pool_fwd(d["x"], d["a"], d["b"], y, d["scales"], other)

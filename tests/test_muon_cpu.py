@@ -35,7 +35,7 @@ def test_calls_in_order_reach_the_device_check():
     (dict(cols=(1 << 30) + 1), 2), (dict(param=None), 1), (dict(param=FAKE + 1), 1), (dict(grad=None), 1),
     (dict(grad=FAKE + 2), 1), (dict(momentum=None), 1), (dict(lr=-1.0), 1), (dict(lr=float("inf")), 1),
     (dict(lr=float("nan")), 1), (dict(beta=1.0), 1), (dict(beta=-0.1), 1), (dict(weight_decay=-1.0), 1),
-    (dict(lr=1.0, weight_decay=1.5), 1), (dict(eps=0.0), 1), (dict(eps=float("nan")), 1),
+    (dict(lr=1.0, weight_decay=1.5), 1), (dict(eps=0.0), 1), (dict(eps=1e-301), 1), (dict(eps=float("nan")), 1),
     (dict(scale=float("inf")), 1), (dict(a=float("nan")), 1), (dict(steps=-1), 1), (dict(steps=11), 1),
     (dict(count=1 << 30), 2),
 ])

@@ -181,3 +181,21 @@ def test_empty_list_and_no_matrices(device):
     fb.muon_step_many([])
     e = torch.empty(0, 4, 8, device="cuda")
     fb.muon_step(e, e.clone(), e.clone())
+
+
+def test_zero_matrix_under_the_smallest_eps(device):
+    """1 / eps^2 leaves the range of f64; the update is still zero."""
+    for shape in ((16, 40), (40, 20)):
+        p, g, m = make(shape, F32, seed=4)
+        g.zero_(), m.zero_()
+        before = p.clone()
+        fb.muon_step(p, g, m, eps=1e-300)
+        assert torch.equal(p, before) and not m.any()
+
+
+def test_the_same_tensor_twice_is_refused(device):
+    p, g, m = make((8, 40), F32)
+    other = make((8, 40), F32, seed=1)
+    for items in ([(p, g, m), (p, g, other[2])], [(p, g, m), (other[0], g, m)], [(p, g, m)] * 2):
+        with pytest.raises(fb.FoundryAttnError):
+            fb.muon_step_many(items)
