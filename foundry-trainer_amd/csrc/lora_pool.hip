@@ -499,8 +499,13 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 // D[column][token]: a wave's step is 64 columns in four products; row 4 q + e of
 // product j is column 32 (j / 2) + 8 q + 4 (j % 2) + e (f32: 16 j + 4 q + e), so
 // that a lane ends with 16-byte runs of its token's row, the four lanes of a row
-// with 64 bytes side by side.  The rows of y and the factor of the wave's next step are
-// loaded before this step's products.
+// with 64 bytes side by side.  Bound by y's bytes after some 5 us of latencies in a
+// row (plan, low, factor, y): reading and writing y alone in this way took 43 us of
+// the 50 that 6000 x 8192 rank 32 takes (196 MB of y, 3.9 TB/s).  The tokens' operand
+// stays in LDS, so that three or four waves fit a SIMD: with it in registers and the
+// next step's loads ahead, two did, 54 us.  Where the factor's rows go through LDS
+// the next step is loaded ahead all the same (AHEAD): 16.5 against 18.5 us at
+// 4096 x 4096 rank 16 (67 MB).
 constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
 constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
@@ -509,7 +514,11 @@ template <typename T, int RB, bool ROWMAJOR, int KIND>
 __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
     constexpr int PITCH = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
-    __shared__ float lowsum[kRows][RB * 16 + 4];
+    constexpr bool AHEAD = !ROWMAJOR;
+    // the tokens' operand, 64 bytes per 16 ranks: bf16 the high parts, then what
+    // they leave; f32 as they are
+    constexpr int LOWROW = RB * 64 + 16;
+    __shared__ __align__(16) char lowrow[kRows * LOWROW];
     __shared__ __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
@@ -593,30 +602,21 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
         for (int b = 0; b < RB; ++b) {
             if (p.low_out && blockIdx.x == 0 && lrow < t.rows)  // the parts' sum, for the backward
                 store_f4(p.low_out + (int64_t)ltoken * r + 16 * b + 4 * h, r - 16 * b - 4 * h, s[b]);
-            *reinterpret_cast<f32x4 *>(&lowsum[lrow][16 * b + 4 * h]) = s[b] * scale;
+            s[b] *= scale;
+            char *d = lowrow + lrow * LOWROW + 64 * b;
+            if constexpr (sizeof(T) == 2) {
+                const float w[8] = {s[b][0], s[b][1], s[b][2], s[b][3], 0.f, 0.f, 0.f, 0.f};
+                u32x4 terms[2];
+                split_terms(w, terms);
+                *reinterpret_cast<u32x2 *>(d + 8 * h) = u32x2{terms[0][0], terms[0][1]};
+                *reinterpret_cast<u32x2 *>(d + 32 + 8 * h) = u32x2{terms[1][0], terms[1][1]};
+            } else {
+                *reinterpret_cast<f32x4 *>(d + 16 * h) = s[b];
+            }
         }
     }
     if (!live) return;
     __syncthreads();
-    // the tokens' operand: bf16 takes the high parts of 16 ranks in lane groups
-    // 0 and 1, what they leave in 2 and 3; f32 ranks 4 q .. + 4
-    u32x4 low[RB][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            const float *src = &lowsum[16 * i + x][16 * b];
-            if constexpr (sizeof(T) == 2) {
-                const f32x4 lo = *reinterpret_cast<const f32x4 *>(src + 8 * (q & 1));
-                const f32x4 hi = *reinterpret_cast<const f32x4 *>(src + 8 * (q & 1) + 4);
-                const float w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                u32x4 terms[2];
-                split_terms(w, terms);
-                low[b][i] = q < 2 ? terms[0] : terms[1];
-            } else {
-                low[b][i] = *reinterpret_cast<const u32x4 *>(src + 4 * q);
-            }
-        }
     char *mine = stage + (ROWMAJOR ? 0 : wave * RB * 16 * PITCH);
     while (c0 < W) {
         u32x4 fc[4][RB], yc[4][NY];
@@ -663,16 +663,21 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
             for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
         const int64_t lo = c0, c = step_base(c0, kUpStep, W) + E * q;
         c0 += step;
-        if (c0 < W) load(c0);
+        if (AHEAD && c0 < W) load(c0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i >= subs) continue;
+            // bf16: lane groups 0 and 1 the high parts of 16 ranks, 2 and 3 the rest; f32: ranks 4 q ..
+            u32x4 low[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+                low[b] = *reinterpret_cast<const u32x4 *>(lowrow + (16 * i + x) * LOWROW + 64 * b + 16 * q);
             f32x4 acc[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b][i], acc[j]);
+                for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b], acc[j]);
             }
             if (16 * i + x >= t.rows) continue;
 #pragma unroll
@@ -689,6 +694,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                 }
             }
         }
+        if (!AHEAD && c0 < W) load(c0);
     }
 }
 
