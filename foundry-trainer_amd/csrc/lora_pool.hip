@@ -11,9 +11,10 @@
 // there is none, so nothing of the index has to come back to the host.
 //   pool_down   64 rows x a range of the wide axis: u or v, f32, over `splits`
 //               ranges that the reader adds in order
-//   pool_up     64 rows x 256 columns: y or dx
-//   pool_grad   a chunk x 256 (f32: 128) columns of dA or dB: straight to the
-//               result where the adapter has one chunk, else a partial sum
+//   pool_up     64 rows x 256 columns or twice that: y
+//   pool_back   dx in the same way, and beside it dA and dB: a chunk x 256 (f32:
+//               128) columns, straight to the result where the adapter has one
+//               chunk, else a partial sum
 //   pool_reduce the partial sums in order, and zeros for adapters without tokens
 // u and v are f32 between the kernels.  bf16 products (v_mfma_f32_16x16x32) take
 // them as sums of bf16 terms, high part first: two terms (2^-17) where the result
@@ -502,27 +503,32 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 // with 64 bytes side by side.  Bound by y's bytes after some 5 us of latencies in a
 // row (plan, low, factor, y): reading and writing y alone in this way took 43 us of
 // the 50 that 6000 x 8192 rank 32 takes (196 MB of y, 3.9 TB/s).  The tokens' operand
-// stays in LDS, so that three or four waves fit a SIMD: with it in registers and the
-// next step's loads ahead, two did, 54 us.  Where the factor's rows go through LDS
-// the next step is loaded ahead all the same (AHEAD): 16.5 against 18.5 us at
-// 4096 x 4096 rank 16 (67 MB).
+// stays in LDS and a step's loads follow the step before, so that three or four
+// waves fit a SIMD: with the operand in registers and the next step's loads ahead,
+// two did, 54 us.
 constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
 constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
 
-template <typename T, int RB, bool ROWMAJOR, int KIND>
-__global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
-    constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
-    constexpr int PITCH = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
-    constexpr bool AHEAD = !ROWMAJOR;
+template <typename T, int RB, bool ROWMAJOR>
+struct UpLds {
+    static constexpr int kPitch = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
     // the tokens' operand, 64 bytes per 16 ranks: bf16 the high parts, then what
     // they leave; f32 as they are
-    constexpr int LOWROW = RB * 64 + 16;
-    __shared__ __align__(16) char lowrow[kRows * LOWROW];
-    __shared__ __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * PITCH];
+    static constexpr int kLowRow = RB * 64 + 16;
+    __align__(16) char lowrow[kRows * kLowRow];
+    __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * kPitch];
+};
+
+// Row tile `at`, the wave steps of block `block` of `blocks`.
+template <typename T, int RB, bool ROWMAJOR, int KIND>
+__device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int block, int blocks,
+                                        UpLds<T, RB, ROWMAJOR> &lds) {
+    constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
+    constexpr int PITCH = UpLds<T, RB, ROWMAJOR>::kPitch, LOWROW = UpLds<T, RB, ROWMAJOR>::kLowRow;
+    char *const lowrow = lds.lowrow;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
-    const int64_t at = grid_tile();
     if (at >= most_tiles(p.T, p.L, kRows)) return;
     int token[4];
     tile_tokens(p, v, at, x, token);
@@ -534,14 +540,14 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     clamp_tokens(t, x, token);
     const int r = p.r, W = p.wide, subs = (t.rows + 15) / 16;
     const bool live = t.adapter >= 0;
-    if (!live && !(p.low_out && blockIdx.x == 0)) return;
+    if (!live && !(p.low_out && block == 0)) return;
     const float scale = live ? p.scale[t.adapter] : 0.f;
     const T *factor = static_cast<const T *>(p.factor) + (int64_t)(live ? t.adapter : 0) * r * W;
     T *out[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = static_cast<T *>(p.y) + token[i] * p.ldy;
-    const int64_t step = (int64_t)gridDim.x * 4 * kUpStep;
-    int64_t c0 = ((int64_t)blockIdx.x * 4 + wave) * kUpStep;
+    const int64_t step = (int64_t)blocks * 4 * kUpStep;
+    int64_t c0 = ((int64_t)block * 4 + wave) * kUpStep;
 
     constexpr int RUN = 4 * E;  // columns of one load of the row's four lanes
     // column of row m of product j, and the first of the lane's load n
@@ -600,7 +606,7 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                         f32x4, load_ranks<KIND>(p.low + ((int64_t)k * p.T + ltoken) * r, 16 * b + 4 * h, r));
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-            if (p.low_out && blockIdx.x == 0 && lrow < t.rows)  // the parts' sum, for the backward
+            if (p.low_out && block == 0 && lrow < t.rows)  // the parts' sum, for the backward
                 store_f4(p.low_out + (int64_t)ltoken * r + 16 * b + 4 * h, r - 16 * b - 4 * h, s[b]);
             s[b] *= scale;
             char *d = lowrow + lrow * LOWROW + 64 * b;
@@ -617,9 +623,9 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
     }
     if (!live) return;
     __syncthreads();
-    char *mine = stage + (ROWMAJOR ? 0 : wave * RB * 16 * PITCH);
+    char *mine = lds.stage + (ROWMAJOR ? 0 : wave * RB * 16 * PITCH);
     while (c0 < W) {
-        u32x4 fc[4][RB], yc[4][NY];
+        u32x4 fc[4][RB];
         if constexpr (ROWMAJOR) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -657,13 +663,8 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
                 }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < NY; ++n) yc[i][n] = y[i][n];
         const int64_t lo = c0, c = step_base(c0, kUpStep, W) + E * q;
         c0 += step;
-        if (AHEAD && c0 < W) load(c0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i >= subs) continue;
@@ -683,19 +684,25 @@ __global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
 #pragma unroll
             for (int n = 0; n < NY; ++n) {
                 if constexpr (sizeof(T) == 2) {
-                    const bf16x8 old = as_bf16x8(yc[i][n]);
+                    const bf16x8 old = as_bf16x8(y[i][n]);
                     bf16x8 o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[e] = f32_to_bf16((float)old[e] + acc[2 * n + e / 4][e % 4]);
                     store16(out[i], c + RUN * n, lo, W, as_u32x4(o));
                 } else {
                     store16(out[i], c + RUN * n, lo, W,
-                            __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, yc[i][n]) + acc[n]));
+                            __builtin_bit_cast(u32x4, __builtin_bit_cast(f32x4, y[i][n]) + acc[n]));
                 }
             }
         }
-        if (!AHEAD && c0 < W) load(c0);
+        if (c0 < W) load(c0);
     }
+}
+
+template <typename T, int RB, int KIND>
+__global__ __launch_bounds__(256) void pool_up_kernel(PoolParams p) {
+    __shared__ UpLds<T, RB, true> lds;
+    up_tile<T, RB, true, KIND>(p, grid_tile(), blockIdx.x, gridDim.x, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -767,11 +774,21 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
                 const int token = lds.token[row + e];
                 const float *src = p.low + (int64_t)(token < 0 ? ~token : token) * r;
 #pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    const float w = src[std::min(16 * b + rank, r - 1)];
-                    low[b][e] = token >= 0 && 16 * b + rank < r ? w : 0.f;
-                }
+                for (int b = 0; b < RB; ++b) low[b][e] = src[std::min(16 * b + rank, r - 1)];
             }
+            for (int k = 1; k < p.splits; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int token = lds.token[row + e];
+                    const float *src = p.low + ((int64_t)k * p.T + (token < 0 ? ~token : token)) * r;
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) low[b][e] += src[std::min(16 * b + rank, r - 1)];
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                    low[b][e] = lds.token[row + e] >= 0 && 16 * b + rank < r ? low[b][e] : 0.f;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
                 u32x4 terms[3];
@@ -784,7 +801,9 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
 #pragma unroll 16
         for (int n = 0; n < RB * 16; ++n) {
             const int i = n * 256 + threadIdx.x, row = i / (RB * 16), rank = i % (RB * 16), token = lds.token[row];
-            const float w = p.low[(int64_t)(token < 0 ? ~token : token) * r + std::min(rank, r - 1)];
+            const float *src = p.low + (int64_t)(token < 0 ? ~token : token) * r + std::min(rank, r - 1);
+            float w = src[0];
+            for (int k = 1; k < p.splits; ++k) w += src[(int64_t)k * p.T * r];
             lds.low[row][rank] = token >= 0 && rank < r ? w : 0.f;
         }
     }
@@ -868,18 +887,33 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
     }
 }
 
-template <typename T, int RB>
-__global__ __launch_bounds__(256) void pool_grad_kernel(PoolParams pa, PoolGradParams ga, PoolParams pb,
+// dx, dA and dB in one launch: grid rows up to dx's row tiles, behind them the
+// gradients' (chunk, column block) pairs one after another.  A launch after
+// another costs some 5 us in which no memory is busy: 4096 x 4096 rank 16 took 17
+// and 16 us in two launches, 30 in this one (x, dy, dx twice: 134 MB, 4.4 TB/s),
+// 33 with the gradients first; 300 tokens 5 and 6.4, 7.3 in one.
+template <typename T, int RB, int KIND>
+__global__ __launch_bounds__(256) void pool_back_kernel(PoolParams px, PoolParams pa, PoolGradParams ga, PoolParams pb,
                                                         PoolGradParams gb) {
-    __shared__ GradLds<T, RB> lds;
+    __shared__ union {
+        GradLds<T, RB> grad;
+        UpLds<T, RB, false> up;
+    } lds;
+    const int64_t tiles = px.y ? most_tiles(px.T, px.L, kRows) : 0, at = grid_tile() - tiles;
+    if (at < 0) {
+        up_tile<T, RB, false, KIND>(px, at + tiles, blockIdx.x, gridDim.x, lds.up);
+        return;
+    }
+    if (!ga.out) return;  // the grid's last rows, of a call for dx alone
     const PlanView v = plan_view(const_cast<int *>(pa.plan), pa.T, pa.L);
+    const int64_t i = at * gridDim.x + blockIdx.x, chunk = i / (ga.blocks + gb.blocks);
+    const int block = (int)(i - chunk * (ga.blocks + gb.blocks));
     Tile t;
-    const int64_t at = grid_tile();
-    if (at >= most_tiles(pa.T, pa.L, kChunk) || !tile_of(pa, v, true, at, t) || t.adapter < 0) return;
-    if ((int)blockIdx.x < ga.blocks)
-        grad_chunk<T, RB>(ga, pa, v, t, blockIdx.x, lds);
+    if (chunk >= most_tiles(pa.T, pa.L, kChunk) || !tile_of(pa, v, true, chunk, t) || t.adapter < 0) return;
+    if (block < ga.blocks)
+        grad_chunk<T, RB>(ga, pa, v, t, block, lds.grad);
     else
-        grad_chunk<T, RB>(gb, pb, v, t, blockIdx.x - ga.blocks, lds);
+        grad_chunk<T, RB>(gb, pb, v, t, block - ga.blocks, lds.grad);
 }
 
 // Adapters of several chunks: the partial sums in order, times the scale;
@@ -902,16 +936,6 @@ __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGrad
         for (int k = 0; k < chunks; ++k) s += load_f4(part + k * size + e, left);
         store_f4(out + e, left, chunks ? s * scale : s);
     }
-}
-
-// u or v: the parts' sum, where no pool_up of it makes that.
-__global__ __launch_bounds__(256) void pool_sum_kernel(const float *low, int splits, int64_t n, float *out) {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    const int left = (int)std::min<int64_t>(4, n - e);
-    if (left <= 0) return;
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) s += load_f4(low + k * n + e, left);
-    store_f4(out + e, left, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -946,39 +970,55 @@ hipError_t down_t(const PoolParams &p, hipStream_t s) {
     }
     return hipGetLastError();
 }
-template <typename T, bool ROWMAJOR, int KIND>
+// Workgroups over a row of pool_up: two steps a wave where one each would not all
+// fit the chip at once (three workgroups a CU)
+int64_t up_blocks(int64_t tiles, int wide) {
+    const int64_t blocks = ((int64_t)wide + 4 * kUpStep - 1) / (4 * kUpStep);
+    return tiles * blocks > 3 * (int64_t)device_cu_count() ? (blocks + 1) / 2 : blocks;
+}
+template <typename T, int KIND>
 hipError_t up_kind(const PoolParams &p, hipStream_t s) {
-    // two steps a wave where one each would not all fit the chip at once (three workgroups a CU)
-    const int64_t tiles = most_tiles(p.T, p.L, kRows), blocks = ((int64_t)p.wide + 4 * kUpStep - 1) / (4 * kUpStep);
-    const int64_t turns = tiles * blocks > 3 * (int64_t)device_cu_count() ? 2 : 1;
-    const dim3 grid = tile_grid((blocks + turns - 1) / turns, tiles), block(256);
+    const int64_t tiles = most_tiles(p.T, p.L, kRows);
+    const dim3 grid = tile_grid(up_blocks(tiles, p.wide), tiles), block(256);
     switch ((p.r + 15) / 16) {
-        case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
-        case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
-        case 3: hipLaunchKernelGGL((pool_up_kernel<T, 3, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
-        default: hipLaunchKernelGGL((pool_up_kernel<T, 4, ROWMAJOR, KIND>), grid, block, 0, s, p); break;
+        case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, KIND>), grid, block, 0, s, p); break;
+        case 2: hipLaunchKernelGGL((pool_up_kernel<T, 2, KIND>), grid, block, 0, s, p); break;
+        case 3: hipLaunchKernelGGL((pool_up_kernel<T, 3, KIND>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((pool_up_kernel<T, 4, KIND>), grid, block, 0, s, p); break;
     }
     return hipGetLastError();
-}
-template <typename T, bool ROWMAJOR>
-hipError_t up_t(const PoolParams &p, hipStream_t s) {
-    switch (rank_kind(p.r)) {
-        case 0: return up_kind<T, ROWMAJOR, 0>(p, s);
-        case 1: return up_kind<T, ROWMAJOR, 1>(p, s);
-        default: return up_kind<T, ROWMAJOR, 2>(p, s);
-    }
 }
 template <typename T>
-hipError_t grad_t(const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb, const PoolGradParams &gb,
-                  hipStream_t s) {
-    const dim3 grid = tile_grid(ga.blocks + gb.blocks, most_tiles(pa.T, pa.L, kChunk)), block(256);
-    switch ((pa.r + 15) / 16) {
-        case 1: hipLaunchKernelGGL((pool_grad_kernel<T, 1>), grid, block, 0, s, pa, ga, pb, gb); break;
-        case 2: hipLaunchKernelGGL((pool_grad_kernel<T, 2>), grid, block, 0, s, pa, ga, pb, gb); break;
-        case 3: hipLaunchKernelGGL((pool_grad_kernel<T, 3>), grid, block, 0, s, pa, ga, pb, gb); break;
-        default: hipLaunchKernelGGL((pool_grad_kernel<T, 4>), grid, block, 0, s, pa, ga, pb, gb); break;
+hipError_t up_t(const PoolParams &p, hipStream_t s) {
+    switch (rank_kind(p.r)) {
+        case 0: return up_kind<T, 0>(p, s);
+        case 1: return up_kind<T, 1>(p, s);
+        default: return up_kind<T, 2>(p, s);
+    }
+}
+template <typename T, int KIND>
+hipError_t back_kind(const PoolParams &px, const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb,
+                     const PoolGradParams &gb, hipStream_t s) {
+    const int64_t tiles = px.y ? most_tiles(px.T, px.L, kRows) : 0;
+    const int64_t pairs = ga.out ? most_tiles(pa.T, pa.L, kChunk) * (ga.blocks + gb.blocks) : 0;
+    const int64_t columns = tiles ? up_blocks(tiles, px.wide) : ga.blocks + gb.blocks;
+    const dim3 grid = tile_grid(columns, tiles + (pairs + columns - 1) / columns), block(256);
+    switch ((px.r + 15) / 16) {
+        case 1: hipLaunchKernelGGL((pool_back_kernel<T, 1, KIND>), grid, block, 0, s, px, pa, ga, pb, gb); break;
+        case 2: hipLaunchKernelGGL((pool_back_kernel<T, 2, KIND>), grid, block, 0, s, px, pa, ga, pb, gb); break;
+        case 3: hipLaunchKernelGGL((pool_back_kernel<T, 3, KIND>), grid, block, 0, s, px, pa, ga, pb, gb); break;
+        default: hipLaunchKernelGGL((pool_back_kernel<T, 4, KIND>), grid, block, 0, s, px, pa, ga, pb, gb); break;
     }
     return hipGetLastError();
+}
+template <typename T>
+hipError_t back_t(const PoolParams &px, const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb,
+                  const PoolGradParams &gb, hipStream_t s) {
+    switch (rank_kind(px.r)) {
+        case 0: return back_kind<T, 0>(px, pa, ga, pb, gb, s);
+        case 1: return back_kind<T, 1>(px, pa, ga, pb, gb, s);
+        default: return back_kind<T, 2>(px, pa, ga, pb, gb, s);
+    }
 }
 
 }  // namespace
@@ -1004,7 +1044,7 @@ size_t pool_fwd_workspace_bytes(const PoolCall &c) {
 
 size_t pool_bwd_workspace_bytes(const PoolCall &c) {
     const int splits = down_splits(c.T, c.L, c.M);
-    return low_bytes(c.T, c.r, splits) + (splits > 1 ? low_bytes(c.T, c.r, 1) : 0) +
+    return low_bytes(c.T, c.r, splits) +
            align256((size_t)grad_slots(c.T, c.L) * c.r * ((size_t)c.K + c.M) * sizeof(float));
 }
 
@@ -1034,7 +1074,7 @@ hipError_t launch_pool_fwd(const PoolCall &c, int dtype, hipStream_t s) {
     p.y = c.y;
     p.ldy = c.ldy;
     p.low_out = p.splits > 1 ? c.u : nullptr;
-    return dtype == 0 ? up_t<bf16, true>(p, s) : up_t<float, true>(p, s);
+    return dtype == 0 ? up_t<bf16>(p, s) : up_t<float>(p, s);
 }
 
 hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
@@ -1045,10 +1085,8 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
     hipError_t e = hipSuccess;
     PoolParams pa = pv, pb = pv;  // the gradients' products
     PoolGradParams ga{}, gb{};
-    // workspace: v's parts, v, the partial gradients
-    float *v = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
-    float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(v) +
-                                            (pv.splits > 1 ? low_bytes(c.T, c.r, 1) : 0));
+    // workspace: v's parts, the partial gradients
+    float *part = reinterpret_cast<float *>(static_cast<char *>(c.work) + low_bytes(c.T, c.r, pv.splits));
     const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
     const int cols = bf ? 256 : 128;
     ga.out = c.da;
@@ -1065,32 +1103,21 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
         pv.factor = c.b;
         pv.wide = c.M;
         if ((e = bf ? down_t<bf16, false>(pv, s) : down_t<float, false>(pv, s)) != hipSuccess) return e;
-        if (c.dx) {
-            PoolParams px = pv;
-            px.factor = c.a;
-            px.wide = c.K;
-            px.y = c.dx;
-            px.ldy = c.lddx;
-            px.low_out = pv.splits > 1 && c.da ? v : nullptr;
-            if ((e = bf ? up_t<bf16, false>(px, s) : up_t<float, false>(px, s)) != hipSuccess) return e;
-        }
-        if (c.da && pv.splits > 1 && !c.dx) {
-            const int64_t n = (int64_t)c.T * c.r;
-            hipLaunchKernelGGL(pool_sum_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, pv.low,
-                               pv.splits, n, v);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-        }
+        PoolParams px = pv;
+        px.factor = c.a;
+        px.wide = c.K;
+        px.y = c.dx;
+        px.ldy = c.lddx;
         pa.x = c.x;
         pa.ldx = c.ldx;
         pa.wide = c.K;
-        pa.low = pv.splits > 1 ? v : pv.low;
-        pa.splits = 1;
         pb.x = c.dy;
         pb.ldx = c.lddy;
         pb.wide = c.M;
         pb.low = c.u;
         pb.splits = 1;
-        if (c.da && (e = bf ? grad_t<bf16>(pa, ga, pb, gb, s) : grad_t<float>(pa, ga, pb, gb, s)) != hipSuccess)
+        if ((c.dx || c.da) &&
+            (e = bf ? back_t<bf16>(px, pa, ga, pb, gb, s) : back_t<float>(px, pa, ga, pb, gb, s)) != hipSuccess)
             return e;
     }
     if (!c.da) return hipSuccess;
