@@ -99,7 +99,9 @@ __device__ __forceinline__ float wave_sum(float s) {
 constexpr int kMaxWaves = 16;
 
 // A row belongs to a group of G waves, P groups to a workgroup.  Wave w of the
-// group holds elements (k * G + w) * 512 + 8 * lane .. + 8 for k < CH.
+// group holds elements (k * G + w) * 512 + 8 * lane .. + 8 for k < CH.  Bound by
+// HBM: 15.7 us at 4096 x 4096 bf16 (67 MB, 4.3 TB/s), 26 to 28 at 32768 x 1024
+// (134 MB, 5 TB/s).
 template <typename T, typename WT, int CH>
 __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p) {
     __shared__ float red[2][kMaxWaves];
@@ -174,7 +176,10 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p)
 
 // Backward: each group takes R rows at a time and keeps its columns' sums of
 // dy * n and dy in registers; the workgroup adds its groups' in order and
-// writes one row of partial sums [2][C].
+// writes one row of partial sums [2][C], so that dw and db cost no second pass
+// over x and dy.  Bound by HBM: 26 us at 4096 x 4096 bf16 (101 MB, 3.9 TB/s), 41 at
+// 32768 x 1024 (201 MB, 4.9 TB/s); without the next rows' loads ahead (AHEAD) more,
+// as the two reductions of a row leave memory idle.
 template <typename T, typename WT, int CH, int R, bool AHEAD>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(LayerNormParams p) {
     __shared__ float red[2][kMaxWaves][2 * R];
@@ -311,7 +316,8 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(LayerNormParams p)
 }
 
 // dw and db: the column sums of the partial rows [count][2][C], 64 columns and
-// 16 interleaved row ranges per workgroup, added in order.
+// 16 interleaved row ranges per workgroup, added in order.  Latency-bound, 4 to
+// 4.7 us: 256 partial rows at C = 4096 are 8 MB.
 __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float *part, int count, int C, float *dw,
                                                                  float *db) {
     __shared__ float red[16][64];

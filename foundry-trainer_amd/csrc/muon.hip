@@ -93,7 +93,10 @@ __device__ __forceinline__ void store4(float *base, int64_t at, int64_t step, in
 
 // Momentum and the chunk's part of u u^T.  Wave w takes every fourth 16-column
 // step of the chunk; lane l holds row 16 b + l % 16 of each of the RB row blocks
-// and the step's columns 4 (l / 16) .. + 4.
+// and the step's columns 4 (l / 16) .. + 4.  Bound by HBM: 51.5 us for the
+// f32 factors of 64 projections 2048 -> 8192 of rank 32, 21 M elements (read g and
+// m, write m: 252 MB, 4.9 TB/s); at rank 64 by the f64 MFMA, 16 us for 8 matrices
+// of 4096 columns.
 template <int RB>
 __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
     constexpr int NT = RB * (RB + 1) / 2;
@@ -167,8 +170,8 @@ __global__ __launch_bounds__(256) void muon_gram_kernel(MuonMany p) {
 // T of one matrix.  Element i of a tile in lane l is (row 4 i + l / 16, column
 // l % 16).  Of up to 2 x 2 tiles each wave owns one (one alone stays in its
 // wave's registers), of more a column of them.  Bound by the latency of the
-// products one after another (four a step, three deep, an MFMA 64 cycles): 64
-// matrices take the time of one.  Only the tiles on and above the diagonal, mirrored
+// products one after another (four a step, three deep, an MFMA 64 cycles): 128
+// matrices of rank 32 take 13.8 us, two of rank 16 6.9.  Only the tiles on and above the diagonal, mirrored
 // in LDS, would be 10 of 16 products at rank 64, but measured 52 us against 47.
 template <int RB>
 __global__ __launch_bounds__(256) void muon_solve_kernel(MuonMany p) {
@@ -341,7 +344,9 @@ __device__ __forceinline__ void store_param4(bf16 *base, int64_t at, int64_t ste
 // Wide matrices (rows contiguous along n): a wave's step is 64 columns, product e
 // those 4 x + e, so that a lane's loads and stores are 4 columns of a row.  Tall
 // ones (contiguous along r): 16 columns, the step's k in the order a lane's 4
-// elements of a column give it.
+// elements of a column give it.  Bound by HBM: 63 us for those 21 M elements (read
+// g, m, p, write p: 336 MB, 5.3 TB/s).  u is formed again from g and m: writing it
+// in the first pass would move as many bytes more.
 template <typename T, int RB, bool WIDE>
 __device__ __forceinline__ void apply_matrix(const MuonMany &p, const Place &at, const float *turn) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
