@@ -1597,6 +1597,8 @@ fa_status fa_lora_pool_bwd(const fa_lora_pool_bwd_args *a, void *stream) {
     if (a->dx) FA_TRY(check_any_view("dx", a->dx, a->ldx, f->tokens, f->in_features, f->dtype));
     if ((a->da == nullptr) != (a->db == nullptr) || !aligned(a->da, 4) || !aligned(a->db, 4))
         return fail(FA_ERR_INVALID_ARG, "da and db must both be given or both NULL, 4-byte aligned");
+    if (a->da && a->dx && f->tokens && (a->dx == f->x || a->dx == a->dy))
+        return fail(FA_ERR_INVALID_ARG, "dx may not be x or dy, which the factors' gradients read");
     fa::PoolCall c = pool_call(f);
     FA_TRY(check_pool_workspace(f, fa::pool_bwd_workspace_bytes(c)));
     c.dy = a->dy;

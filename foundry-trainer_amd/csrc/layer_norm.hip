@@ -151,7 +151,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p)
             }
         }
         const float rstd = 1.f / sqrtf(group_sum(q, red[1]) * inv_c + p.eps);
-        if (!live) continue;  // its group has met every barrier of this round
+        if (!live) continue;  // its group has met every barrier of this pass
         T *y = static_cast<T *>(p.y) + row * p.ldy;
 #pragma unroll
         for (int k = 0; k < CH; ++k) {

@@ -486,7 +486,8 @@ typedef struct fa_lora_pool_bwd_args {
 
 /* da_i = scale_i sum_t (B_i^T dy[t]) x[t]^T and db_i = scale_i sum_t dy[t]
  * u[t]^T over the tokens of adapter i (zero for adapters without any), and the
- * adapters' share of the input's gradient.  Deterministic. */
+ * adapters' share of the input's gradient.  No output may overlap an input or
+ * another output.  Deterministic. */
 size_t fa_lora_pool_bwd_workspace_size(const fa_lora_pool_bwd_args *args);
 fa_status fa_lora_pool_bwd(const fa_lora_pool_bwd_args *args, void *stream);
 

@@ -21,7 +21,7 @@ def args(**kw):
 
 
 def bwd_args(fwd=None, **kw):
-    a = _abi.LoraPoolBwdArgs(fwd=args(**(fwd or {})), dy=FAKE, ldy=17, da=FAKE, db=FAKE, dx=FAKE, ldx=33)
+    a = _abi.LoraPoolBwdArgs(fwd=args(**(fwd or {})), dy=FAKE, ldy=17, da=FAKE, db=FAKE, dx=2 * FAKE, ldx=33)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -35,7 +35,7 @@ bwd = lambda f=None, **kw: lib().fa_lora_pool_bwd(ctypes.byref(bwd_args(f, **kw)
 def test_calls_in_order_reach_the_device_check():
     assert fwd() == fwd(tokens=1, ldx=0) == fwd(rank=64, adapters=2048) == _abi.FA_ERR_NO_DEVICE
     assert fwd(tokens=0, x=None, y=None, u=None) == bwd(dict(tokens=0, x=None, u=None), dy=None) == _abi.FA_ERR_NO_DEVICE
-    assert bwd() == bwd(dx=None) == bwd(da=None, db=None) == _abi.FA_ERR_NO_DEVICE
+    assert bwd() == bwd(dx=None) == bwd(da=None, db=None) == bwd(da=None, db=None, dx=FAKE) == _abi.FA_ERR_NO_DEVICE
     assert lib().fa_lora_pool_plan(FAKE, 40, 3, FAKE, 1 << 20, None) == _abi.FA_ERR_NO_DEVICE
     assert lib().fa_lora_pool_plan(None, 0, 3, FAKE, 1 << 20, None) == _abi.FA_ERR_NO_DEVICE
 
@@ -57,6 +57,7 @@ def test_refusals_of_one():
     assert fwd(in_features=1 << 20, ldx=1 << 20, workspace=None) == fwd(in_features=1 << 20, ldx=1 << 20,
                                                                         workspace_bytes=16) == bad
     assert bwd(dy=None) == bwd(ldy=16) == bwd(da=None) == bwd(db=FAKE + 1) == bwd(ldx=32) == bad
+    assert bwd(dx=FAKE) == bwd(dict(x=2 * FAKE)) == bad  # dx over dy, over x
     assert bwd(dict(workspace=None)) == bwd(dict(workspace=FAKE + 64)) == bwd(dict(workspace_bytes=64)) == bad
     assert lib().fa_lora_pool_fwd(None, None) == lib().fa_lora_pool_bwd(None, None) == bad
 

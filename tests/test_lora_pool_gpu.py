@@ -218,6 +218,21 @@ def test_no_tokens_and_frozen_factors(device):
     assert torch.equal(da, want["da"]) and torch.equal(db, want["db"])
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_parts_of_the_backward(device, dt):
+    """The gradients alone and dx alone have the whole backward's bits, where v
+    comes in parts (wide dy) and where dx is narrower or wider than the factors."""
+    for K, M in ((40, 1030), (1030, 300), (2100, 2100)):
+        d = make(300, 3, K, M, 20, dt, seed=K)
+        want = run_and_check(d)
+        plan = fa.lora_pool_plan(d["index"], 3)
+        da, db = fa.lora_pool_bwd(d["x"], d["a"], d["b"], want["u"], d["dy"], d["scales"], plan)
+        assert torch.equal(da, want["da"]) and torch.equal(db, want["db"])
+        dx = d["dx"].clone()
+        fa.lora_pool_bwd(d["x"], d["a"], d["b"], want["u"], d["dy"], d["scales"], plan, dx=dx, want_factors=False)
+        assert torch.equal(dx, want["dx"])
+
+
 def test_autograd_matches_differences(device):
     """The wrapper's gradients against central differences in 64 bits (h = 1e-4)."""
     d = make(12, 3, 20, 10, 4, F32, seed=29)

@@ -21,7 +21,7 @@ def test_struct_layouts_match_header(tmp_path):
     for cname, py in STRUCTS.items():
         lines.append(f'printf("{cname} size %zu\\n", sizeof({cname}));')
         lines += [f'printf("{cname} {field} %zu\\n", offsetof({cname}, {field}));' for field, _ in py._fields_]
-    lines += [f'printf("limits rank %d\\n", FA_MUON_MAX_RANK);', f'printf("limits steps %d\\n", FA_MUON_MAX_STEPS);',
+    lines += ['printf("limits rank %d\\n", FA_MUON_MAX_RANK);', 'printf("limits steps %d\\n", FA_MUON_MAX_STEPS);',
               "return 0;}"]
     src, exe = tmp_path / "layout.c", tmp_path / "layout"
     src.write_text("\n".join(lines))
