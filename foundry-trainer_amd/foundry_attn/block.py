@@ -46,7 +46,7 @@ import torch
 
 from . import _abi, gemm_tuning
 from ._abi import FoundryAttnError, check, lib
-from .ops import (_dtype_code, _f32, _ptr, _stream, attn_bwd, attn_bwd_workspace_bytes, attn_fwd, lora_bwd, lora_down,
+from .ops import (_as_rows, _dtype_code, _f32, _ptr, _stream, attn_bwd, attn_bwd_workspace_bytes, attn_fwd, lora_bwd, lora_down,
                   lora_fwd, lora_grad,
                   lora_grad_many,
                   lora_up, qk_prologue_bwd_multi, qk_prologue_multi, rope_tables)
@@ -196,7 +196,7 @@ def layer_norm_bwd(x, dy, weight, mean, rstd, dres=None, out=None, want_dweight:
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _as_rows(x)
         y, mean, rstd = layer_norm_fwd(x2, weight, bias, eps)
         ctx.save_for_backward(x2, weight, mean, rstd)
         ctx.bias_dtype = None if bias is None else bias.dtype

@@ -746,10 +746,18 @@ def lora_pool_bwd(x, a, b, u, dy, scales, plan: LoraPoolPlan, dx=None, want_fact
     return da, db
 
 
+def _as_rows(x):
+    """x [..., C] as rows [N, C] with contiguous elements; copied where its
+    layout has none (an expanded or transposed x)."""
+    rows = x.reshape(-1, x.shape[-1])
+    plain = (rows.shape[1] == 1 or rows.stride(1) == 1) and (rows.shape[0] <= 1 or rows.stride(0) >= rows.shape[1])
+    return rows if plain else rows.contiguous()
+
+
 class _LoraPoolFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, base, scales, plan):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _as_rows(x)
         y = base.clone(memory_format=torch.contiguous_format)
         a, b = a.contiguous(), b.contiguous()
         u = lora_pool_fwd(x2, a, b, y.view(-1, y.shape[-1]), scales, plan)

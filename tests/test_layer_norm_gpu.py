@@ -168,6 +168,20 @@ def test_autograd_matches_differences(device):
             assert abs(t.grad[at].item() - want) < 1e-4 * (1 + abs(want)), (k, at)
 
 
+@pytest.mark.parametrize("layout", ["expanded", "transposed"])
+def test_autograd_of_inputs_without_rows(device, layout):
+    """A broadcast or transposed x and upstream gradient: what a copy gives."""
+    x0, w0, b0, dy, _ = make(20, 20, F32, F32, seed=6)
+    view = (lambda t: t[:1].expand(20, 20)) if layout == "expanded" else (lambda t: t.t())
+    got = []
+    for lay in (view, lambda t: view(t).contiguous()):
+        x, w, b = (t.clone().requires_grad_() for t in (x0, w0, b0))
+        y = fb.layer_norm(lay(x), w, b)
+        y.backward(lay(dy))
+        got.append([y, x.grad, w.grad, b.grad])
+    assert all(torch.equal(p, q) for p, q in zip(*got)) and got[0][1].any()
+
+
 def test_other_stream_and_graph(device):
     x, w, b, dy, _ = make(300, 1030, BF, BF, seed=6)
     want = run(x, w, b, dy, None)

@@ -255,6 +255,26 @@ def test_autograd_matches_differences(device):
         assert abs(leaves[k].grad[at].item() - want) < 1e-4 * (1 + abs(want)), (k, at)
 
 
+@pytest.mark.parametrize("layout", ["expanded", "transposed"])
+def test_autograd_of_inputs_without_rows(device, layout):
+    """A broadcast or transposed x, base and upstream gradient: what a copy gives."""
+    d = make(30, 3, 24, 24, 4, F32, seed=31)
+    view = (lambda t: t[:1].expand(30, 24)) if layout == "expanded" else (lambda t: t[:24].t().contiguous().t())
+    index = d["index"] if layout == "expanded" else d["index"][:24].contiguous()
+    plan, got = fa.lora_pool_plan(index, 3), []
+    for lay in (view, lambda t: view(t).contiguous()):
+        x, a, b, y = (d[k].clone().requires_grad_() for k in ("x", "a", "b", "y"))
+        out = fa.lora_pool(lay(x), a, b, lay(y), d["scales"], plan)
+        out.backward(lay(d["dy"]))
+        got.append([out, x.grad, a.grad, b.grad, y.grad])
+    assert all(torch.equal(p, q) for p, q in zip(got[0][:4], got[1])) and got[0][1].any()
+    # base's gradient is the upstream one itself, which autograd sums over a broadcast's 30 rows in an order that
+    # follows the layout: n additions err by (n - 1) 2^-24 of the sum of magnitudes at most, in either order
+    p, q = got[0][4], got[1][4]
+    mags = torch.zeros_like(p).copy_(view(d["dy"]).abs().sum(0) if layout == "expanded" else view(d["dy"]).abs().sum())
+    assert ((p - q).abs() <= 2 * 29 * 2.0 ** -24 * mags * (1 + 1e-5)).all()
+
+
 def test_plan_changed_before_the_backward(device):
     d = make(12, 3, 20, 10, 4, F32, seed=29)
     plan = fa.lora_pool_plan(d["index"], 3)
