@@ -84,8 +84,8 @@ __device__ __forceinline__ int wave_scan(int x) {
 // `token` they begin.  The lanes of a wave that hold the same adapter find each
 // other by one ballot per bit of its number: 64 tokens of 48 adapters took 5 us
 // by one ballot per adapter.  Latency-bound: the index is read once, into LDS
-// where it fits, and the sums over adapters are one wave's.  3.6 us for 1 token
-// (a launch that does nothing takes about 2), 4.1 for 64, 6.8 for 4096, 8.8 for 6000;
+// where it fits, and the sums over adapters are one wave's.  3.7 us for 1 token
+// (a launch that does nothing takes about 2), 4.3 for 64, 6.4 for 4096, 7.3 for 6000;
 // it serves every projection of the step, and one workgroup needs no second launch.
 constexpr int kPlanKept = 8192;
 __host__ __device__ inline bool plan_keeps(int T, int L) { return T <= kPlanKept && L <= 1024; }
@@ -102,10 +102,14 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
     const int64_t share = (((int64_t)T + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
     const int64_t t0 = wave * share, t1 = std::min<int64_t>(T, t0 + share);
     const bool kept = plan_keeps(T, L);
-    if (kept)
+    if (kept && T > 0) {
+        int w[kPlanKept / 1024];  // all loads before the first wait
+#pragma unroll
+        for (int k = 0; k < kPlanKept / 1024; ++k) w[k] = index[std::min(k * 1024 + tid, T - 1)];
 #pragma unroll
         for (int k = 0; k < kPlanKept / 1024; ++k)
-            if (k * 1024 + tid < T) idx[k * 1024 + tid] = index[k * 1024 + tid];
+            if (k * 1024 + tid < T) idx[k * 1024 + tid] = w[k];
+    }
     for (int i = tid; i < kPlanWaves * A; i += 1024) hist[i] = 0;
     __syncthreads();
     auto adapter_of = [&](int64_t t) {
