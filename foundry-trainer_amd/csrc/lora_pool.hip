@@ -384,7 +384,7 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TE
 // A wave takes every fourth 128-byte step of the range, two operands a lane; the
 // four waves' sums are added through LDS.  64 rows a workgroup, so that the factor
 // is read from L2 once per 64 rows.  Bound by x's bytes after some 5 us of
-// latencies in a row: 10.6 to 12 us at 4096 x 4096 rank 16 (34 MB), 12.6 at
+// latencies in a row: 10.6 to 12 us at 4096 x 4096 rank 16 (34 MB), 12 at
 // 6000 x 2048 rank 32 (25 MB).
 template <typename T, int RB, bool ROWMAJOR>
 __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
@@ -512,10 +512,10 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 // that a lane ends with 16-byte runs of its token's row, the four lanes of a row
 // with 64 bytes side by side.  Bound by y's bytes after some 5 us of latencies in a
 // row (plan, low, factor, y): reading and writing y alone in this way took 43 us of
-// the 50 that 6000 x 8192 rank 32 takes (196 MB of y, 3.9 TB/s).  The tokens' operand
+// the 48 that 6000 x 8192 rank 32 takes (196 MB of y, 4.1 TB/s).  The tokens' operand
 // stays in LDS and a step's loads follow the step before, so that three or four
 // waves fit a SIMD: with the operand in registers and the next step's loads ahead,
-// two did, 54 us.
+// two did, 54 us against 50 (low then in four parts).
 constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
 constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
@@ -956,11 +956,11 @@ __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGrad
 // ---------------------------------------------------------------------------
 // Ranges of the wide axis: about a workgroup a CU, a power of two so that the
 // waves' steps divide evenly, none under 256 columns.  us of down + up, 6000 x 2048
-// -> 8192 rank 32: one range 64, two 60, three 64, four 61, eight 65; 4096 x 4096
-// rank 16: two 33, four 30, eight 30.
+// -> 8192 rank 32 (107 tiles): one range 63, two 59, four 63, eight 68; of both
+// down, up and back, 4096 x 4096 rank 16 (69 tiles): one 103, two 82, four 74, eight 78.
 int down_splits(int T, int L, int W) {
     const int64_t tiles = std::max<int64_t>(1, most_tiles(T, L, kRows));
-    const int64_t want = ((int64_t)device_cu_count() * 4 / 3 + tiles - 1) / tiles;
+    const int64_t want = ((int64_t)device_cu_count() + tiles - 1) / tiles;
     int64_t splits = 1;
     while (2 * splits <= std::min<int64_t>(std::min<int64_t>(want, 64), W / 256)) splits *= 2;
     return (int)splits;
