@@ -23,7 +23,6 @@ listed() holds fixed cases, draw() further ones of the same ranges: from a
 single decoded token to a batch of 8192, pools of one to 64 adapters of ranks
 1 to 64, widths from 64 to 8192, odd ones among them, bf16 and f32.
 """
-import functools
 import math
 import os
 import sys
@@ -202,7 +201,6 @@ def prepare(case, seed):
 # ---------------------------------------------------------------------------
 # the framework's calls
 # ---------------------------------------------------------------------------
-@functools.lru_cache(maxsize=None)  # a program imports them once
 def _calls():
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "foundry-trainer_amd")
     if pkg not in sys.path:
