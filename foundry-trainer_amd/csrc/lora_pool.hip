@@ -17,9 +17,10 @@
 //               chunk, else a partial sum
 //   pool_reduce the partial sums in order, and zeros for adapters without tokens
 // u and v are f32 between the kernels.  bf16 products (v_mfma_f32_16x16x32) take
-// them as sums of bf16 terms, high part first: two terms (2^-17) where the result
-// is rounded to bf16, three (2^-25) where it stays f32.  f32 products are
-// v_mfma_f32_16x16x4.  No atomics: the same bits every time.
+// them as the sum of three bf16 terms, high part first, which holds all 24 bits:
+// with two (2^-17) y and dx round to another bf16 value than the f32 product's one
+// time in a thousand.  f32 products are v_mfma_f32_16x16x4.  No atomics: the same
+// bits every time.
 #include <algorithm>
 #include <type_traits>
 
@@ -523,9 +524,9 @@ constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
 template <typename T, int RB, bool ROWMAJOR>
 struct UpLds {
     static constexpr int kPitch = sizeof(T) == 2 ? kUpPitch : kUpPitchF;
-    // the tokens' operand, 64 bytes per 16 ranks: bf16 the high parts, then what
-    // they leave; f32 as they are
-    static constexpr int kLowRow = RB * 64 + 16;
+    // the tokens' operand of 16 ranks: bf16 its three terms and zeros, 32 bytes
+    // each (the operands of two products); f32 as they are, 64 bytes
+    static constexpr int kLow = sizeof(T) == 2 ? 128 : 64, kLowRow = RB * kLow + 16;
     __align__(16) char lowrow[kRows * kLowRow];
     __align__(16) char stage[ROWMAJOR ? 16 : 4 * RB * 16 * kPitch];
 };
@@ -536,6 +537,7 @@ __device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int blo
                                         UpLds<T, RB, ROWMAJOR> &lds) {
     constexpr int E = 16 / sizeof(T), NY = 16 / E;  // elements of a load, loads of a lane's 16 columns
     constexpr int PITCH = UpLds<T, RB, ROWMAJOR>::kPitch, LOWROW = UpLds<T, RB, ROWMAJOR>::kLowRow;
+    constexpr int LOW = UpLds<T, RB, ROWMAJOR>::kLow;
     char *const lowrow = lds.lowrow;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
     const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
@@ -619,13 +621,15 @@ __device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int blo
             if (p.low_out && block == 0 && lrow < t.rows)  // the parts' sum, for the backward
                 store_f4(p.low_out + (int64_t)ltoken * r + 16 * b + 4 * h, r - 16 * b - 4 * h, s[b]);
             s[b] *= scale;
-            char *d = lowrow + lrow * LOWROW + 64 * b;
+            char *d = lowrow + lrow * LOWROW + LOW * b;
             if constexpr (sizeof(T) == 2) {
                 const float w[8] = {s[b][0], s[b][1], s[b][2], s[b][3], 0.f, 0.f, 0.f, 0.f};
-                u32x4 terms[2];
+                u32x4 terms[3];
                 split_terms(w, terms);
-                *reinterpret_cast<u32x2 *>(d + 8 * h) = u32x2{terms[0][0], terms[0][1]};
-                *reinterpret_cast<u32x2 *>(d + 32 + 8 * h) = u32x2{terms[1][0], terms[1][1]};
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    *reinterpret_cast<u32x2 *>(d + 32 * k + 8 * h) = u32x2{terms[k][0], terms[k][1]};
+                *reinterpret_cast<u32x2 *>(d + 96 + 8 * h) = u32x2{0, 0};
             } else {
                 *reinterpret_cast<f32x4 *>(d + 16 * h) = s[b];
             }
@@ -678,17 +682,22 @@ __device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int blo
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i >= subs) continue;
-            // bf16: lane groups 0 and 1 the high parts of 16 ranks, 2 and 3 the rest; f32: ranks 4 q ..
-            u32x4 low[RB];
-#pragma unroll
-            for (int b = 0; b < RB; ++b)
-                low[b] = *reinterpret_cast<const u32x4 *>(lowrow + (16 * i + x) * LOWROW + 64 * b + 16 * q);
+            // bf16: lane groups 0 and 1 the first terms of 16 ranks, 2 and 3 the second, in
+            // another product the third and zeros; f32: ranks 4 q ..
+            constexpr int PARTS = LOW / 64;
             f32x4 acc[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b], acc[j]);
+            for (int k = 0; k < PARTS; ++k) {
+                u32x4 low[RB];
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+                    low[b] = *reinterpret_cast<const u32x4 *>(lowrow + (16 * i + x) * LOWROW + LOW * b + 64 * k + 16 * q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b], acc[j]);
             }
             if (16 * i + x >= t.rows) continue;
 #pragma unroll
