@@ -359,7 +359,8 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 acc) {
     return acc;
 }
 
-// v as a sum of bf16 terms: term k rounds what the terms before it left.
+// v as a sum of bf16 terms: term k rounds what the terms before it left.  A finite
+// value past the largest bf16 is cut instead, one that is not finite has one term.
 template <int TERMS>
 __device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TERMS]) {
     float rest[8];
@@ -371,10 +372,33 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], u32x4 (&out)[TE
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             t[j] = f32_to_bf16(rest[j]);
+            if (k == 0 && __builtin_isinf((float)t[j]) && __builtin_isfinite(rest[j]))
+                t[j] = __builtin_bit_cast(bf16, (uint16_t)(__builtin_bit_cast(uint32_t, rest[j]) >> 16));
             rest[j] = __builtin_isfinite((float)t[j]) ? rest[j] - (float)t[j] : 0.f;
         }
         out[k] = as_u32x4(t);
     }
+}
+// A product's other operand, for the terms after the first: an infinity or NaN has
+// met the whole value's in the first one already, and would make a NaN with a
+// later term that is zero or of the other sign.
+__device__ __forceinline__ u32x4 finite_only(u32x4 v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t top = ((v[k] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;  // exponents of all ones
+        v[k] &= ~((top >> 15) * 0xffffu);
+    }
+    return v;
+}
+// Whether some lane's values hold a NaN, or infinities of both signs.
+template <int N>
+__device__ __forceinline__ bool any_nan(const f32x4 (&v)[N]) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += v[j][e];
+    return __ballot(s != s) != 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -699,6 +723,23 @@ __device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int blo
 #pragma unroll
                     for (int b = 0; b < RB; ++b) acc[j] = mfma16<T>(fc[j][b], low[b], acc[j]);
             }
+            if constexpr (sizeof(T) == 2)
+                if (any_nan(acc)) {  // perhaps of an infinity in the factor; the same sums, in the same order
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+                        for (int b = 0; b < RB; ++b) {
+                            const u32x4 low = *reinterpret_cast<const u32x4 *>(lowrow + (16 * i + x) * LOWROW + LOW * b +
+                                                                               64 * k + 16 * q);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                acc[j] = mfma16<T>(k == 0 && q < 2 ? fc[j][b] : finite_only(fc[j][b]), low, acc[j]);
+                                __builtin_amdgcn_sched_barrier(0);  // one operand's registers at a time
+                            }
+                        }
+                }
             if (16 * i + x >= t.rows) continue;
 #pragma unroll
             for (int n = 0; n < NY; ++n) {
@@ -830,11 +871,13 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
     }
     __syncthreads();
     f32x4 acc[RB][E];
+    // FINITE: the terms after the first take no infinities of the rows
+    auto products = [&](auto finite) __attribute__((always_inline)) {
+        constexpr bool FINITE = decltype(finite)::value;
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
+        for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (any)
+            for (int j = 0; j < E; ++j) acc[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int s = pair; s < steps; s += 2) {
             u32x4 w[ROWS];
 #pragma unroll
@@ -852,10 +895,11 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
                     bf16x8 col;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) col[e] = as_bf16x8(w[e])[j];
+                    const bf16x8 rest = FINITE ? as_bf16x8(finite_only(as_u32x4(col))) : col;
 #pragma unroll
                     for (int b = 0; b < RB; ++b)
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) acc[b][j] = mfma_16x16x32(low[b][k], col, acc[b][j]);
+                        for (int k = 0; k < 3; ++k) acc[b][j] = mfma_16x16x32(low[b][k], k ? rest : col, acc[b][j]);
                 }
             } else {
 #pragma unroll
@@ -870,6 +914,19 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
                 }
             }
         }
+    };
+    if (any) {
+        products(std::false_type{});
+        if constexpr (sizeof(T) == 2) {
+            bool nan = false;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) nan |= any_nan(acc[b]);
+            if (nan) {
+                if (pair < steps) load_wide(pair);
+                products(std::true_type{});
+            }
+        }
+    }
     __syncthreads();
     if (pair == 1)
 #pragma unroll
