@@ -779,6 +779,9 @@ class _LoraPoolFn(torch.autograd.Function):
 
 def lora_pool(x, a, b, base, scales, plan: LoraPoolPlan):
     """Differentiable base + adapter term of lora_pool_fwd: x [..., K], base
-    [..., M] the shared projection's output; gradients for x, a, b and base.
-    plan.update between this and its backward is an error torch reports."""
+    [..., M] the shared projection's output; gradients for x, a, b and base, none
+    for scales, which are refused where autograd would want one.  plan.update
+    between this and its backward is an error torch reports."""
+    if torch.is_grad_enabled() and scales.requires_grad:
+        raise FoundryAttnError(_abi.FA_ERR_UNSUPPORTED, "scales require a gradient, which lora_pool does not compute")
     return _LoraPoolFn.apply(x, a, b, base, scales, plan)
