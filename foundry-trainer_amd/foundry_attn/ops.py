@@ -677,8 +677,8 @@ def _pool_rows(t, shape: tuple, like, name: str):
     return t
 
 
-def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u) -> tuple:
-    """LoraPoolArgs' values in field order, up to y."""
+def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u=None) -> tuple:
+    """u, a new one where not given, and LoraPoolArgs' values in field order, up to y."""
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3 or not x.is_cuda:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "x must be [T, K] on the device, a [L, r, K], b [L, M, r]")
     T, K = x.shape
@@ -694,12 +694,14 @@ def _pool_args(x, a, b, scales, plan: LoraPoolPlan, u) -> tuple:
     if plan.tokens != T or plan.adapters != L or plan.data.device != dev:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"the plan is of {plan.tokens} tokens and {plan.adapters} "
                                                         f"adapters, the call of {T} and {L}")
-    if u.shape != (T, r) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
-        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"u must be contiguous float32 [{T}, {r}] on {dev}")
     if K > 1 and x.stride(1) != 1:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "x must have contiguous rows")
-    return (_dtype_code(x), T, K, M, r, L, x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
-            plan.data.data_ptr(), plan.data.numel(), u.data_ptr())
+    if u is None:
+        u = torch.empty((T, r), dtype=torch.float32, device=dev)
+    elif u.shape != (T, r) or u.dtype != torch.float32 or not u.is_contiguous() or u.device != dev:
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, f"u must be contiguous float32 [{T}, {r}] on {dev}")
+    return u, (_dtype_code(x), T, K, M, r, L, x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
+               plan.data.data_ptr(), plan.data.numel(), u.data_ptr())
 
 
 @functools.lru_cache(maxsize=4096)
@@ -716,8 +718,7 @@ def lora_pool_fwd(x, a, b, y, scales, plan: LoraPoolPlan):
     tokens without one stay.  x [T, K], a [L, r, K], b [L, M, r], y [T, M], scales
     [L] f32; rank 1..64 (pad lower ranks with zeros).  Returns u = A_i x (f32
     [T, r], zero rows without an adapter) for the backward."""
-    u = torch.empty((x.shape[0], a.shape[1]), dtype=torch.float32, device=x.device)
-    head = _pool_args(x, a, b, scales, plan, u)
+    u, head = _pool_args(x, a, b, scales, plan)
     _pool_rows(y, (head[1], head[3]), x, "y")
     stream = _stream(x)
     need = _pool_bytes(x.get_device(), False, *head[:6])
@@ -730,7 +731,7 @@ def lora_pool_bwd(x, a, b, u, dy, scales, plan: LoraPoolPlan, dx=None, want_fact
     """(da, db) in f32, [L, r, K] and [L, M, r], of lora_pool_fwd for the upstream
     gradient dy (zero for adapters without tokens; None each without
     want_factors); dx[t] += scales[i] A_i^T (B_i^T dy[t]) when given."""
-    head = _pool_args(x, a, b, scales, plan, u)
+    head = _pool_args(x, a, b, scales, plan, u)[1]
     _pool_rows(dy, (head[1], head[3]), x, "dy")
     if dx is not None:
         _pool_rows(dx, (head[1], head[2]), x, "dx")
