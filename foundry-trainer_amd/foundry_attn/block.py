@@ -398,6 +398,8 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
     param is [rows, cols] or [n, rows, cols] (n matrices, each by itself, e.g. a
     pool's factors), bf16 or f32, min(rows, cols) <= 64; grad and momentum are
     f32 of its shape; all contiguous, the params of one dtype on one device.
+    What is written may not overlap: every param and momentum is its own, and no
+    gradient is one of them (items may share a gradient, which is only read).
     scale: default sqrt(max(1, rows / cols)) of each."""
     items = list(items)
     if not items:
@@ -407,7 +409,7 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
     if not first.is_cuda:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "params must be device tensors")
     ca, cb, cc = (float(v) for v in coeffs)
-    packed, count, seen = [], 0, set()
+    packed, count, seen, grads = [], 0, set(), set()
     for p, g, m in items:
         if p.dim() not in (2, 3) or not p.is_contiguous() or p.dtype != first.dtype or p.device != dev:
             raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG,
@@ -419,6 +421,7 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
         if p.dim() == 3 and p.shape[0] == 0:
             continue
         seen |= {p.data_ptr(), m.data_ptr()}
+        grads.add(g.data_ptr())
         rows, cols = p.shape[-2:]
         sc = math.sqrt(max(1.0, rows / max(cols, 1))) if scale is None else float(scale)
         packed.append(_pack_muon(code, p.shape[0] if p.dim() == 3 else 1, rows, cols, p.data_ptr(), g.data_ptr(),
@@ -429,6 +432,8 @@ def muon_step_many(items, lr: float = 0.02, beta: float = 0.95, weight_decay: fl
         return
     if len(seen) != 2 * count:
         raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "a param or momentum is listed twice")
+    if not seen.isdisjoint(grads):
+        raise FoundryAttnError(_abi.FA_ERR_INVALID_ARG, "a gradient is a param or momentum of the step")
     arr, stream = b"".join(packed), _stream(first)
     need = max(_abi.entry("fa_muon_step_many_workspace_size", ctypes.c_int32, size=True)(arr, count), 256)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
