@@ -27,6 +27,7 @@
 #include "fa_device.hpp"
 #include "fa_kernels.hpp"
 #include "fa_lds.hpp"
+#include "pool_plan.hpp"
 
 namespace fa {
 namespace {
@@ -34,41 +35,14 @@ namespace {
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-constexpr int kRows = 64;     // of a row tile
-constexpr int kChunk = 256;   // rows of a gradient chunk: whole tiles
+constexpr int kRows = kPoolRows, kChunk = kPoolChunk;
 constexpr int kPlanWaves = 16;
+using Tile = PoolTile;
+using PlanView = PoolPlanView;
 
 // ---------------------------------------------------------------------------
-// the plan: int32 words
+// the plan
 // ---------------------------------------------------------------------------
-struct Tile {
-    int tile, rows, adapter, slot;  // rows token[64 * tile .. + rows); adapter -1: none
-};
-struct PlanView {
-    int *head;    // tiles, chunks, T, L
-    int *count;   // [L] tokens of each adapter
-    int *slot0;   // [L] its first partial gradient; -1: none (at most one chunk)
-    Tile *tiles, *chunks;
-    int *token;   // sorted by adapter, those without one last; each adapter begins a tile
-};
-__host__ __device__ inline int64_t most_tiles(int64_t T, int64_t L, int rows) {
-    return (T + rows - 1) / rows + (L + 1 < T ? L + 1 : T);
-}
-__host__ __device__ inline int64_t round4(int64_t x) { return (x + 3) & ~int64_t(3); }
-__host__ __device__ inline int64_t plan_words(int64_t T, int64_t L) {
-    return 4 + 2 * round4(L) + (4 + kRows) * most_tiles(T, L, kRows) + 4 * most_tiles(T, L, kChunk);
-}
-__host__ __device__ inline PlanView plan_view(int *p, int64_t T, int64_t L) {
-    PlanView v;
-    v.head = p;
-    v.count = p + 4;
-    v.slot0 = v.count + round4(L);
-    v.tiles = reinterpret_cast<Tile *>(v.slot0 + round4(L));
-    v.chunks = v.tiles + most_tiles(T, L, kRows);
-    v.token = reinterpret_cast<int *>(v.chunks + most_tiles(T, L, kChunk));
-    return v;
-}
-
 // Inclusive sum over the lanes before and at this one.
 __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
@@ -99,7 +73,7 @@ __global__ __launch_bounds__(1024) void pool_plan_kernel(const int *index, int T
     __shared__ int total[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, A = L + 1;
     int *rows = hist + kPlanWaves * A, *tiles0 = rows + L + 2, *chunks0 = tiles0 + L + 2, *idx = chunks0 + L + 2;
-    const PlanView v = plan_view(plan, T, L);
+    const PlanView v = pool_plan_view(plan, T, L);
     const int64_t share = (((int64_t)T + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;
     const int64_t t0 = wave * share, t1 = std::min<int64_t>(T, t0 + share);
     const bool kept = plan_keeps(T, L);
@@ -237,14 +211,11 @@ __device__ __forceinline__ bool tile_of(const PoolParams &p, const PlanView &v, 
     const u32x4 head = *reinterpret_cast<const u32x4 *>(v.head);
     const u32x4 w = *reinterpret_cast<const u32x4 *>((chunk ? v.chunks : v.tiles) + i);
     t = __builtin_bit_cast(Tile, w);
-    const int n = (int)(chunk ? head[1] : head[0]), most = chunk ? kChunk : kRows;
-    return (int)head[2] == p.T && (int)head[3] == p.L && i < n && t.tile >= 0 && t.rows > 0 && t.rows <= most &&
-           (int64_t)t.tile + (t.rows + kRows - 1) / kRows <= most_tiles(p.T, p.L, kRows) && t.adapter < p.L;
+    return pool_tile_fits((int)(chunk ? head[1] : head[0]), (int)head[2], (int)head[3], t, i, chunk, p.T, p.L);
 }
 // The token in entry `at` of the plan's list; 0 where it holds no token.
 __device__ __forceinline__ int token_at(const PoolParams &p, const PlanView &v, int64_t at) {
-    const int row = v.token[at];
-    return (unsigned)row < (unsigned)p.T ? row : 0;
+    return pool_row(v.token[at], p.T);
 }
 // Its tokens, for a lane that reads row 16 i + x of a row tile in its i-th load:
 // rows past the end read the block's first (and are not written).
@@ -416,9 +387,9 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), STEP = 8 * E;
     __shared__ f32x4 sum[4][RB][4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
-    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    const PlanView v = pool_plan_view(const_cast<int *>(p.plan), p.T, p.L);
     const int64_t at = grid_tile();
-    if (at >= most_tiles(p.T, p.L, kRows)) return;
+    if (at >= pool_most_tiles(p.T, p.L, kRows)) return;
     int token[4];
     tile_tokens(p, v, at, x, token);
     Tile t;
@@ -564,8 +535,8 @@ __device__ __forceinline__ void up_tile(const PoolParams &p, int64_t at, int blo
     constexpr int LOW = UpLds<T, RB, ROWMAJOR>::kLow;
     char *const lowrow = lds.lowrow;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4;
-    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
-    if (at >= most_tiles(p.T, p.L, kRows)) return;
+    const PlanView v = pool_plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    if (at >= pool_most_tiles(p.T, p.L, kRows)) return;
     int token[4];
     tile_tokens(p, v, at, x, token);
     // four threads a row: its ranks 4 h .. of every 16, the parts in order
@@ -939,9 +910,9 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
     for (int b = 0; b < RB; ++b)
 #pragma unroll
         for (int j = 0; j < E; ++j) acc[b][j] += lds.sum[wave][b][j][lane];
-    const int slot = t.slot >= 0 ? v.slot0[t.adapter] + t.slot : -1;
-    if (slot >= g.slots || (t.slot >= 0 && slot < 0)) return;  // not of a plan that this library made
-    float *out = slot >= 0 ? g.part + slot * (int64_t)r * W : g.out + t.adapter * (int64_t)r * W;
+    const int64_t slot = pool_grad_place(t.slot, v.slot0[t.adapter], g.slots);
+    if (slot == kPoolNowhere) return;  // not of a plan that this library made
+    float *out = slot >= 0 ? g.part + slot * r * W : g.out + t.adapter * (int64_t)r * W;
     const float scale = slot >= 0 ? 1.f : p.scale[t.adapter];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
@@ -977,17 +948,17 @@ __global__ __launch_bounds__(256) void pool_back_kernel(PoolParams px, PoolParam
         GradLds<T, RB> grad;
         UpLds<T, RB, false> up;
     } lds;
-    const int64_t tiles = px.y ? most_tiles(px.T, px.L, kRows) : 0, at = grid_tile() - tiles;
+    const int64_t tiles = px.y ? pool_most_tiles(px.T, px.L, kRows) : 0, at = grid_tile() - tiles;
     if (at < 0) {
         up_tile<T, RB, false, KIND>(px, at + tiles, blockIdx.x, gridDim.x, lds.up);
         return;
     }
     if (!ga.out) return;  // the grid's last rows, of a call for dx alone
-    const PlanView v = plan_view(const_cast<int *>(pa.plan), pa.T, pa.L);
+    const PlanView v = pool_plan_view(const_cast<int *>(pa.plan), pa.T, pa.L);
     const int64_t i = at * gridDim.x + blockIdx.x, chunk = i / (ga.blocks + gb.blocks);
     const int block = (int)(i - chunk * (ga.blocks + gb.blocks));
     Tile t;
-    if (chunk >= most_tiles(pa.T, pa.L, kChunk) || !tile_of(pa, v, true, chunk, t) || t.adapter < 0) return;
+    if (chunk >= pool_most_tiles(pa.T, pa.L, kChunk) || !tile_of(pa, v, true, chunk, t) || t.adapter < 0) return;
     if (block < ga.blocks)
         grad_chunk<T, RB>(ga, pa, v, t, block, lds.grad);
     else
@@ -1000,10 +971,10 @@ __global__ __launch_bounds__(256) void pool_back_kernel(PoolParams px, PoolParam
 __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGradParams ga, PoolGradParams gb,
                                                           int64_t na, int64_t nb) {
     const int a = blockIdx.x;
-    const PlanView v = plan_view(const_cast<int *>(p.plan), p.T, p.L);
-    const int n = v.count[a], first = v.slot0[a], chunks = (n + kChunk - 1) / kChunk;
-    if (v.head[2] != p.T || v.head[3] != p.L || chunks == 1) return;
-    if (chunks > 1 && (first < 0 || first > ga.slots - chunks)) return;
+    const PlanView v = pool_plan_view(const_cast<int *>(p.plan), p.T, p.L);
+    const int first = v.slot0[a];
+    const int64_t chunks = pool_partials(v.head[2], v.head[3], v.count[a], first, ga.slots, p.T, p.L);
+    if (chunks < 0) return;
     const float scale = p.scale[a];
     const int64_t size = blockIdx.z ? nb : na;
     const float *part = (blockIdx.z ? gb.part : ga.part) + first * size;
@@ -1012,7 +983,7 @@ __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGrad
         const int left = (int)std::min<int64_t>(4, size - e);
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int k = 0; k < chunks; ++k) s += load_f4(part + k * size + e, left);
+        for (int64_t k = 0; k < chunks; ++k) s += load_f4(part + k * size + e, left);
         store_f4(out + e, left, chunks ? s * scale : s);
     }
 }
@@ -1025,22 +996,18 @@ __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGrad
 // -> 8192 rank 32 (107 tiles): one range 63, two 59, four 63, eight 68; of both
 // down, up and back, 4096 x 4096 rank 16 (69 tiles): one 103, two 82, four 74, eight 78.
 int down_splits(int T, int L, int W) {
-    const int64_t tiles = std::max<int64_t>(1, most_tiles(T, L, kRows));
+    const int64_t tiles = std::max<int64_t>(1, pool_most_tiles(T, L, kRows));
     const int64_t want = ((int64_t)device_cu_count() + tiles - 1) / tiles;
     int64_t splits = 1;
     while (2 * splits <= std::min<int64_t>(std::min<int64_t>(want, 64), W / 256)) splits *= 2;
     return (int)splits;
 }
-// Partial gradients: the chunks of adapters with more than one, all full but each
-// adapter's last
-int64_t grad_slots(int T, int L) { return (int64_t)T / kChunk + std::min<int64_t>(L, (int64_t)T / (kChunk + 1)); }
-
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 size_t low_bytes(int T, int r, int splits) { return align256((size_t)splits * T * r * sizeof(float)); }
 
 template <typename T, bool ROWMAJOR>
 hipError_t down_t(const PoolParams &p, hipStream_t s) {
-    const dim3 grid = tile_grid(p.splits, most_tiles(p.T, p.L, kRows)), block(256);
+    const dim3 grid = tile_grid(p.splits, pool_most_tiles(p.T, p.L, kRows)), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_down_kernel<T, 1, ROWMAJOR>), grid, block, 0, s, p); break;
         case 2: hipLaunchKernelGGL((pool_down_kernel<T, 2, ROWMAJOR>), grid, block, 0, s, p); break;
@@ -1057,7 +1024,7 @@ int64_t up_blocks(int64_t tiles, int wide) {
 }
 template <typename T, int KIND>
 hipError_t up_kind(const PoolParams &p, hipStream_t s) {
-    const int64_t tiles = most_tiles(p.T, p.L, kRows);
+    const int64_t tiles = pool_most_tiles(p.T, p.L, kRows);
     const dim3 grid = tile_grid(up_blocks(tiles, p.wide), tiles), block(256);
     switch ((p.r + 15) / 16) {
         case 1: hipLaunchKernelGGL((pool_up_kernel<T, 1, KIND>), grid, block, 0, s, p); break;
@@ -1078,8 +1045,8 @@ hipError_t up_t(const PoolParams &p, hipStream_t s) {
 template <typename T, int KIND>
 hipError_t back_kind(const PoolParams &px, const PoolParams &pa, const PoolGradParams &ga, const PoolParams &pb,
                      const PoolGradParams &gb, hipStream_t s) {
-    const int64_t tiles = px.y ? most_tiles(px.T, px.L, kRows) : 0;
-    const int64_t pairs = ga.out ? most_tiles(pa.T, pa.L, kChunk) * (ga.blocks + gb.blocks) : 0;
+    const int64_t tiles = px.y ? pool_most_tiles(px.T, px.L, kRows) : 0;
+    const int64_t pairs = ga.out ? pool_most_tiles(pa.T, pa.L, kChunk) * (ga.blocks + gb.blocks) : 0;
     const int64_t columns = tiles ? up_blocks(tiles, px.wide) : ga.blocks + gb.blocks;
     const dim3 grid = tile_grid(columns, tiles + (pairs + columns - 1) / columns), block(256);
     switch ((px.r + 15) / 16) {
@@ -1108,7 +1075,7 @@ hipError_t prepare_pool_kernels() {
                                plan_lds_words(kPlanKept + 1, kPoolMaxAdapters) * (int)sizeof(int));
 }
 
-size_t pool_plan_bytes(int T, int L) { return (size_t)plan_words(T, L) * sizeof(int); }
+size_t pool_plan_bytes(int T, int L) { return (size_t)pool_plan_words(T, L) * sizeof(int); }
 
 hipError_t launch_pool_plan(const int *index, int T, int L, int *plan, hipStream_t s) {
     const size_t lds = (size_t)plan_lds_words(T, L) * sizeof(int);
@@ -1124,7 +1091,7 @@ size_t pool_fwd_workspace_bytes(const PoolCall &c) {
 size_t pool_bwd_workspace_bytes(const PoolCall &c) {
     const int splits = down_splits(c.T, c.L, c.M);
     return low_bytes(c.T, c.r, splits) +
-           align256((size_t)grad_slots(c.T, c.L) * c.r * ((size_t)c.K + c.M) * sizeof(float));
+           align256((size_t)pool_grad_slots(c.T, c.L) * c.r * ((size_t)c.K + c.M) * sizeof(float));
 }
 
 static PoolParams pool_params(const PoolCall &c) {
@@ -1169,7 +1136,7 @@ hipError_t launch_pool_bwd(const PoolCall &c, int dtype, hipStream_t s) {
     const int64_t na = (int64_t)c.r * c.K, nb = (int64_t)c.r * c.M;
     const int cols = bf ? 256 : 128;
     ga.out = c.da;
-    ga.slots = gb.slots = (int)grad_slots(c.T, c.L);
+    ga.slots = gb.slots = (int)pool_grad_slots(c.T, c.L);
     ga.part = part;
     ga.blocks = (c.K + cols - 1) / cols;
     gb.out = c.db;
