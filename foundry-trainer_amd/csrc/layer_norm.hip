@@ -100,8 +100,9 @@ constexpr int kMaxWaves = 16;
 
 // A row belongs to a group of G waves, P groups to a workgroup.  Wave w of the
 // group holds elements (k * G + w) * 512 + 8 * lane .. + 8 for k < CH.  Bound by
-// HBM: 15.7 us at 4096 x 4096 bf16 (67 MB, 4.3 TB/s), 26 to 28 at 32768 x 1024
-// (134 MB, 5 TB/s).
+// HBM: 15.6 us at 4096 x 4096 bf16 (67 MB, 4.3 TB/s), 26 to 30 at 32768 x 1024
+// (134 MB, 4.5 to 5 TB/s), f32 4096 x 4096 31 (134 MB).  Under 512 columns lanes are
+// idle: 100000 rows take 35 us at 64 columns and at 128 (26 and 51 MB).
 template <typename T, typename WT, int CH>
 __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p) {
     __shared__ float red[2][kMaxWaves];
@@ -177,9 +178,13 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_kernel(LayerNormParams p)
 // Backward: each group takes R rows at a time and keeps its columns' sums of
 // dy * n and dy in registers; the workgroup adds its groups' in order and
 // writes one row of partial sums [2][C], so that dw and db cost no second pass
-// over x and dy.  Bound by HBM: 26 us at 4096 x 4096 bf16 (101 MB, 3.9 TB/s), 41 at
-// 32768 x 1024 (201 MB, 4.9 TB/s); without the next rows' loads ahead (AHEAD) more,
-// as the two reductions of a row leave memory idle.
+// over x and dy.  Bound by HBM: 26 us at 4096 x 4096 bf16 (101 MB, 3.9 TB/s), 41 to
+// 44 at 32768 x 1024 (201 MB, 4.6 to 4.9 TB/s), 59 at 2048 x 16384 (201 MB); without
+// the next rows' loads ahead (AHEAD) more, as the two reductions of a row leave
+// memory idle.  Not so at four chunks a lane, C > 16384: of the sums of 32 columns,
+// the weights and the rows, 208 to 314 registers a lane lie in scratch memory, and
+// 2048 x 16392 takes 274 us, 1024 x 32768 322 (201 MB both; f32 254).  Under 512
+// columns lanes are idle: 100000 rows take 50 us at 64 columns and at 128.
 template <typename T, typename WT, int CH, int R, bool AHEAD>
 __global__ __launch_bounds__(1024) void layer_norm_bwd_kernel(LayerNormParams p) {
     __shared__ float red[2][kMaxWaves][2 * R];
@@ -338,8 +343,8 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float *pa
 // Waves per row of C elements with CH chunks of 512 per wave.
 int group_waves(int C, int ch) { return (C + 512 * ch - 1) / (512 * ch); }
 
-// Rows at a time of a group of waves, and whether the next are loaded ahead:
-// what 128 VGPRs hold.
+// Rows at a time of a group of waves, and whether the next are loaded ahead: what
+// the 128 VGPRs of 1024 threads hold at one and two chunks a lane (four do not fit).
 template <typename T, int CH>
 constexpr int kBwdRows = sizeof(T) == 2 && CH == 1 ? 2 : 1;
 
@@ -350,6 +355,8 @@ struct BwdShape {
 // reach every CU otherwise.
 BwdShape bwd_shape(int N, int C, int dtype) {
     BwdShape s{};
+    // as few chunks a lane as 16 waves allow; us, bf16: 4096 x 8192 (one) 49, x 8200 (two)
+    // 56; 2048 x 16384 (two) 59, x 16392 (four) 274
     s.ch = C <= 8192 ? 1 : C <= 16384 ? 2 : 4;
     s.G = group_waves(C, s.ch);
     const int64_t rows = dtype == 0 && s.ch == 1 ? 2 : 1, cus = device_cu_count();
@@ -361,7 +368,8 @@ BwdShape bwd_shape(int N, int C, int dtype) {
 template <typename T, typename WT>
 hipError_t fwd_t(LayerNormParams p, hipStream_t s) {
     // us: 32768 x 1024 bf16 25.6 with two chunks a wave and 8 waves a workgroup, 27.4 with 4, 30.6 with
-    // one chunk (2 waves a row); 4096 x 4096 15.6 with two chunks, 17.8 with one, 16.1 with four
+    // one chunk (2 waves a row); 4096 x 4096 15.6 with two chunks, 17.8 with one, 16.1 with four;
+    // 4096 x 8192 (two) 32, x 8200 (four) 39
     const int ch = p.C <= 512 ? 1 : p.C <= 8192 ? 2 : 4;
     p.G = group_waves(p.C, ch);
     const int P = std::max(1, 8 / p.G);

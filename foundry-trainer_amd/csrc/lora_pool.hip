@@ -58,10 +58,14 @@ __device__ __forceinline__ int wave_scan(int x) {
 // first counts its tokens of adapter a (a = L: none), then holds where in
 // `token` they begin.  The lanes of a wave that hold the same adapter find each
 // other by one ballot per bit of its number: 64 tokens of 48 adapters took 5 us
-// by one ballot per adapter.  Latency-bound: the index is read once, into LDS
-// where it fits, and the sums over adapters are one wave's.  3.7 us for 1 token
-// (a launch that does nothing takes about 2), 4.3 for 64, 6.4 for 4096, 7.3 for 6000;
-// it serves every projection of the step, and one workgroup needs no second launch.
+// by one ballot per adapter.  Latency-bound: the sums over adapters are one wave's,
+// and up to kPlanKept tokens the index is read once, eight words a thread in flight
+// together, and kept in LDS; of more tokens it is read twice, one step of 64 a wave
+// ahead.  12 adapters, whole requests (token by token): 8192 tokens 7.5 us (9.5),
+// 8193 9.4 (12.8), 13312 12, 65536 53.  3.7 us for 1 token (a launch that does
+// nothing takes about 2), 4.4 for 64, 6.1 for 4096; it serves every projection of
+// the step, and one workgroup needs no second launch.  More than 8192 would fit the
+// LDS beside few adapters, at more registers for the words in flight: not tried.
 constexpr int kPlanKept = 8192;
 __host__ __device__ inline bool plan_keeps(int T, int L) { return T <= kPlanKept && L <= 1024; }
 __host__ __device__ inline int plan_lds_words(int T, int L) {
@@ -381,7 +385,9 @@ __device__ __forceinline__ bool any_nan(const f32x4 (&v)[N]) {
 // four waves' sums are added through LDS.  64 rows a workgroup, so that the factor
 // is read from L2 once per 64 rows.  Bound by x's bytes after some 5 us of
 // latencies in a row: 10.6 to 12 us at 4096 x 4096 rank 16 (34 MB), 12 at
-// 6000 x 2048 rank 32 (25 MB).
+// 6000 x 2048 rank 32 (25 MB).  At ranks over 32 one wave a SIMD is left by the
+// registers (f32 v over 48), and bf16 v spills 13 of them at ranks over 48:
+// 4096 x 4096 rank 64 takes 18 us for u and 21 for v.
 template <typename T, int RB, bool ROWMAJOR>
 __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
     constexpr int E = 16 / sizeof(T), STEP = 8 * E;
@@ -508,10 +514,11 @@ __global__ __launch_bounds__(256) void pool_down_kernel(PoolParams p) {
 // that a lane ends with 16-byte runs of its token's row, the four lanes of a row
 // with 64 bytes side by side.  Bound by y's bytes after some 5 us of latencies in a
 // row (plan, low, factor, y): reading and writing y alone in this way took 43 us of
-// the 48 that 6000 x 8192 rank 32 takes (196 MB of y, 4.1 TB/s).  The tokens' operand
-// stays in LDS and a step's loads follow the step before, so that three or four
-// waves fit a SIMD: with the operand in registers and the next step's loads ahead,
-// two did, 54 us against 50 (low then in four parts).
+// the 48 that 6000 x 8192 rank 32 takes (196 MB of y, 4.1 TB/s; rank 64 66 us).  The
+// tokens' operand stays in LDS and a step's loads follow the step before: with the
+// operand in registers and the next step's loads ahead it took 54 us against 50 (low
+// then in four parts).  Waves a SIMD: bf16 four up to rank 16, three up to 32, two
+// above; f32 two.
 constexpr int kUpStep = 64;                   // columns of a wave's step
 constexpr int kUpPitch = kUpStep * 2 + 8;     // bytes of a staged bf16 factor row: 4 rows x 4 column groups hit distinct banks
 constexpr int kUpPitchF = kUpStep * 4 + 16;   // the same, f32
@@ -942,8 +949,13 @@ __device__ __forceinline__ void grad_chunk(const PoolGradParams &g, const PoolPa
 // dx, dA and dB in one launch: grid rows up to dx's row tiles, behind them the
 // gradients' (chunk, column block) pairs one after another.  A launch after
 // another costs some 5 us in which no memory is busy: 4096 x 4096 rank 16 took 17
-// and 16 us in two launches, 30 in this one (x, dy, dx twice: 134 MB, 4.4 TB/s),
-// 33 with the gradients first; 300 tokens 5 and 6.4, 7.3 in one.
+// and 16 us in two launches, 30 in this one (x, dy, dx twice: 134 MB), 33 with the
+// gradients first; 300 tokens 5 and 6.4, 7.3 in one.  Infinities kept, it takes 32
+// (4.2 TB/s) and 7.9.  Both parts share the registers and the larger LDS, the
+// gradients': three waves a SIMD in bf16 up to rank 16, two up to 32, one above (f32
+// two up to rank 32, one above), also for dx.  4096 x 4096 bf16: rank 32 41 us, 48
+// 65, 64 77; 2048 x 2048 f32: rank 16 29, 64 110.  Two launches were not measured
+// at these ranks.
 template <typename T, int RB, int KIND>
 __global__ __launch_bounds__(256) void pool_back_kernel(PoolParams px, PoolParams pa, PoolGradParams ga, PoolParams pb,
                                                         PoolGradParams gb) {
@@ -970,7 +982,7 @@ __global__ __launch_bounds__(256) void pool_back_kernel(PoolParams px, PoolParam
 
 // Adapters of several chunks: the partial sums in order, times the scale;
 // adapters without tokens: zeros.  grid (adapters, groups of 1024 elements, dA or dB).
-// Latency-bound: 4.8 us for 20 chunks of 4 adapters at 4096 x 4096 rank 16 (10 MB).
+// Latency-bound: 5.1 us for 20 chunks of 4 adapters at 4096 x 4096 rank 16 (10 MB).
 __global__ __launch_bounds__(256) void pool_reduce_kernel(PoolParams p, PoolGradParams ga, PoolGradParams gb,
                                                           int64_t na, int64_t nb) {
     const int a = blockIdx.x;

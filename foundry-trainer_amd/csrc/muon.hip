@@ -4,6 +4,8 @@
 //   m = beta * m + g;   u = nesterov ? g + beta * m : m
 //   X_0 = u / (|u|_F + eps);   X_k+1 = a X_k + (b S + c S^2) X_k,  S = X_k X_k^T
 //   p = p * (1 - lr * decay) - lr * scale * X_steps
+// (the optimiser published as Muon, Jordan and others, 2024; the iteration is of
+// Newton-Schulz type, its usual coefficients the caller's to pass).
 // Every X_k is T_k X_0 with T_k a polynomial in G_0 = X_0 X_0^T, an r x r matrix:
 //   Q_k = a I + b G_k + c G_k^2,   G_k+1 = Q_k G_k Q_k,   T_k+1 = Q_k T_k,
 // so the long side is passed over twice, once for u u^T and once for T u, and
@@ -462,7 +464,11 @@ int row_blocks(const MuonMany &p) {
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Columns of a chunk of the long side: by the matrix alone, so that its bits
-// do not depend on what else the call holds.
+// do not depend on what else the call holds.  Short chunks fill the chip from one
+// matrix, long ones halve the parts that the solve adds up.  us of the three launches,
+// rank 32 f32, chunks of 256 and 512: one 4096 x 32 matrix and its pair 28 and 35, of
+// 8192 30 and 36, of 65536 65 and 56, of 2^20 1075 and 773; 128 matrices of 2048 and
+// 8192 126 and 133.  The two meet between 8192 and 65536 columns.
 int chunk_columns(int n) { return n <= 4096 ? 256 : 512; }
 
 // Where everything lies in the workspace; 0 if a launch would be too large.

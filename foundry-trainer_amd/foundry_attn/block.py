@@ -385,6 +385,7 @@ def adamw_step_many(items, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps:
     check(lib().fa_adamw_step_many(arr, len(items), _stream(items[0][0])))
 
 
+# of the method as published: Muon, Jordan and others, 2024
 MUON_COEFFS = (3.4445, -4.7750, 2.0315)
 
 

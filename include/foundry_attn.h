@@ -466,9 +466,12 @@ typedef struct fa_lora_pool_args {
 /* y[t] += scale_i B_i (A_i x[t]); rows of tokens without an adapter stay as
  * they are.  Any sizes and strides: rows and factors need their element's
  * alignment only.  No output may overlap an input or another output (y may
- * overlap x, which is read first).  Deterministic.  A plan of other tokens or adapters, or
- * memory that is no plan, gives wrong results but leads to no access outside
- * the call's tensors. */
+ * overlap x, which is read first).  Deterministic: the same call gives the same
+ * bits every time; the order of u's and v's sums goes by the numbers of tokens
+ * and adapters, so that a token's last bits may differ in another batch.  u is
+ * f32 in the products, bf16 results are rounded once.  A plan of other tokens or
+ * adapters, or memory that is no plan, gives wrong results but leads to no access
+ * outside the call's tensors. */
 size_t fa_lora_pool_fwd_workspace_size(const fa_lora_pool_args *args);
 fa_status fa_lora_pool_fwd(const fa_lora_pool_args *args, void *stream);
 

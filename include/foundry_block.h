@@ -283,7 +283,8 @@ typedef struct fa_muon_args {
  * gets the same bits whatever else the call holds.  One
  * workspace of fa_muon_step_many_workspace_size bytes (0 for invalid
  * arguments), 256-byte aligned.  No reference counterpart (its optimiser is
- * AdamW, lib.rs:477-510). */
+ * AdamW, lib.rs:477-510); the method is the one published as Muon (Jordan and
+ * others, 2024). */
 size_t fa_muon_step_many_workspace_size(const fa_muon_args *args, int32_t count);
 fa_status fa_muon_step_many(const fa_muon_args *args, int32_t count, void *workspace, size_t workspace_bytes,
                             void *stream);
