@@ -276,8 +276,8 @@ typedef struct fa_muon_args {
  *   p = p (1 - lr weight_decay) - lr scale X
  * (X transposed where rows > cols).  The Gram matrix and the iteration are f64,
  * the rest is f32, p is rounded once.  A matrix of zeros keeps a zero update;
- * one with a NaN or infinity gets NaN all over (with steps = 0 a NaN does, an
- * infinity in its own place).  All tensors share dtype, lr, beta, weight_decay,
+ * one with a NaN or infinity gets NaN all over (with steps = 0 an infinity
+ * makes NaN of the row or column of the short side's length that holds it).  All tensors share dtype, lr, beta, weight_decay,
  * eps, a, b, c, steps and nesterov.  No param or momentum may overlap anything
  * else of the call; gradients are only read, and may be shared.  Each matrix
  * gets the same bits whatever else the call holds.  One
