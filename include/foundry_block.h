@@ -277,12 +277,13 @@ typedef struct fa_muon_args {
  * (X transposed where rows > cols).  The Gram matrix and the iteration are f64,
  * the rest is f32, p is rounded once.  A matrix of zeros keeps a zero update;
  * one with a NaN or infinity gets NaN all over (with steps = 0 an infinity
- * makes NaN of the row or column of the short side's length that holds it).  All tensors share dtype, lr, beta, weight_decay,
- * eps, a, b, c, steps and nesterov.  No param or momentum may overlap anything
- * else of the call; gradients are only read, and may be shared.  Each matrix
- * gets the same bits whatever else the call holds.  One
- * workspace of fa_muon_step_many_workspace_size bytes (0 for invalid
- * arguments), 256-byte aligned.  No reference counterpart (its optimiser is
+ * makes NaN of the row or column of the short side's length that holds it).
+ * All tensors share dtype, lr, beta, weight_decay, eps, a, b, c, steps and
+ * nesterov.  No param or momentum may overlap anything else of the call;
+ * gradients are only read, and may be shared.  Each matrix gets the same bits
+ * whatever else the call holds.  One workspace of
+ * fa_muon_step_many_workspace_size bytes (0 for invalid arguments), 256-byte
+ * aligned.  No reference counterpart (its optimiser is
  * AdamW, lib.rs:477-510); the method is the one published as Muon (Jordan and
  * others, 2024). */
 size_t fa_muon_step_many_workspace_size(const fa_muon_args *args, int32_t count);
